@@ -13,7 +13,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libh2x.so")
 
 H2X_MAX_DIMS = 6
-F32, F64 = 0, 1
+F32, F64, BF16, F16 = 0, 1, 2, 3
+MAX_AXES = 4
+ROTARY_HALVES, ROTARY_NEIGHBOURS = 0, 1
 LHS, RHS = 0, 1
 HALO_GRID_MAX_RANKS = 16
 SHUFFLE_DIRECT_MAX_RANKS = 64
@@ -168,6 +170,28 @@ class CopyAuditReport(ctypes.Structure):
     ]
 
 
+class TokenStrides(ctypes.Structure):
+    """struct h2x_token_strides"""
+    _fields_ = [("sample", c_int64), ("token", c_int64), ("head", c_int64)]
+
+
+class Rotary(ctypes.Structure):
+    """struct h2x_rotary"""
+    _fields_ = [("dtype", c_int32), ("pairing", c_int32), ("head_dim", c_int32), ("heads", c_int32), ("samples", c_int32),
+                ("num_axes", c_int32), ("tokens", c_int64), ("axis_pairs", c_int32 * MAX_AXES),
+                ("positions_sample_stride", c_int64), ("positions_axis_stride", c_int64), ("x", TokenStrides),
+                ("y", TokenStrides)]
+
+
+class Attention(ctypes.Structure):
+    """struct h2x_attention"""
+    _fields_ = [("dtype", c_int32), ("head_dim", c_int32), ("samples", c_int32), ("query_heads", c_int32),
+                ("key_heads", c_int32), ("reserved", c_int32), ("queries", c_int64), ("keys", c_int64),
+                ("window_left", c_int64), ("window_right", c_int64), ("scale", c_double), ("q", TokenStrides),
+                ("k", TokenStrides), ("v", TokenStrides), ("o", TokenStrides), ("d_o", TokenStrides), ("dq", TokenStrides),
+                ("dk", TokenStrides), ("dv", TokenStrides)]
+
+
 # name -> (restype, argtypes); every symbol include/h2x.h declares.
 SIGNATURES = {
     "h2x_abi_version": (c_int, []),
@@ -307,6 +331,19 @@ SIGNATURES = {
                                          c_int, c_void_p]),
     "h2x_shuffle_unpack_batched": (c_int, [POINTER(c_void_p), POINTER(c_void_p),
                                            POINTER(c_void_p), c_int, c_void_p]),
+    "h2x_layer_norm_forward": (c_int, [c_int, c_int, c_size_t, c_int, POINTER(TensorGeometry), POINTER(TensorGeometry), c_void_p,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_double, c_void_p]),
+    "h2x_layer_norm_workspace_bytes": (c_size_t, [c_int, c_size_t, c_int]),
+    "h2x_layer_norm_backward": (c_int, [c_int, c_int, c_size_t, c_int, POINTER(TensorGeometry), POINTER(TensorGeometry),
+                                        POINTER(TensorGeometry), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                        c_void_p, c_void_p, c_void_p, c_void_p]),
+    "h2x_rotary_apply": (c_int, [POINTER(Rotary), c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
+    "h2x_attention_forward_workspace_bytes": (c_size_t, [POINTER(Attention)]),
+    "h2x_attention_forward": (c_int, [POINTER(Attention), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                      c_void_p, c_void_p]),
+    "h2x_attention_backward_workspace_bytes": (c_size_t, [POINTER(Attention)]),
+    "h2x_attention_backward": (c_int, [POINTER(Attention), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,373 @@
+// Attention, backward (include/h2x.h has the formulas; h2x_attention.hpp how the kernels are built).
+//
+// The probabilities are recomputed from the scores and the logarithms of the forward pass, in two passes: one over blocks of queries
+// makes dq (and delta), one over blocks of keys dk and dv.  Each output is summed by the wave that writes it, in a fixed order; the
+// price is that scores and d_o v^T are made twice, seven products in place of five.
+#include "h2x_attention.hpp"
+
+namespace h2x
+{
+namespace attention
+{
+namespace
+{
+
+// Rows of a tile that passes through LDS: 16 KB of 128 16-bit or 32-bit elements.
+template <typename T>
+constexpr int kTileRows = sizeof(T) == 2 ? 64 : 32;
+
+template <typename T>
+struct Args
+{
+    const T *q, *k, *v, *o, *d_o;
+    const float* logsumexp;
+    T *dq, *dk, *dv;
+    // of each row: its logarithm in units of log2 (the largest number where the row is empty), and delta
+    float *log2_sum, *delta;
+    Strides qs, ks, vs, os, d_os, dqs, dks, dvs;
+    Masks masks;
+    float scale, scale_log2;
+    int dim, query_heads, group, blocks;
+    uint32_t total; // workgroups that have work
+};
+
+// Sum of products of two fragments' elements, over both halves.
+template <typename T, int DP>
+__device__ __forceinline__ float dot(const Fragment<T, DP>& a, const Fragment<T, DP>& b)
+{
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < Tile<T, DP>::kChunks / 2; ++c)
+    {
+        const AVec<T, Tile<T, DP>::kPerChunk> x = __builtin_bit_cast(decltype(x), a.chunk[c]), y = __builtin_bit_cast(decltype(x), b.chunk[c]);
+#pragma unroll
+        for (int i = 0; i < Tile<T, DP>::kPerChunk; ++i)
+            sum = __builtin_fmaf(static_cast<float>(x.v[i]), static_cast<float>(y.v[i]), sum);
+    }
+    return halves_sum(sum);
+}
+
+// dq, and what the other pass needs of each row.  As in the forward pass, the waves of a workgroup take 32 queries of a head each.
+template <typename T, int DP, bool Whole>
+__global__ void __launch_bounds__(kThreads) attention_dq_kernel(const Args<T> a)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    constexpr int KT = kTileRows<T>, kTileBytes = KT * Tile<T, DP>::kRowBytes;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
+    const uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
+    if (id >= a.total)
+        return;
+    const int block = a.blocks - 1 - id % a.blocks; // (the longest first under a causal mask)
+    const int head = id / a.blocks % a.query_heads, n = id / a.blocks / a.query_heads;
+    const int lane = threadIdx.x & (kWaveSize - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    const Sample sample = sample_of(a.masks, n);
+
+    const int block_first = block * (kWaves * kRows), block_end = min(block_first + kWaves * kRows, sample.queries);
+    const int first = block_first + wave * kRows, i = first + (lane & 31);
+    const int last = min(first + kRows, sample.queries) - 1;
+    int from = 0, tiles = 0;
+    if (block_first < block_end)
+    {
+        from = sample.first_key(block_first);
+        tiles = (max(sample.end_key(block_end - 1) - from, 0) + KT - 1) / KT;
+    }
+    const T* const k = a.k + n * a.ks.sample + (head / a.group) * a.ks.head;
+    const T* const v = a.v + n * a.vs.sample + (head / a.group) * a.vs.head;
+    const int k_bytes = static_cast<int>(a.ks.token * sizeof(T)), v_bytes = static_cast<int>(a.vs.token * sizeof(T));
+    const auto load = [&](int tile) {
+        const int at = from + tile * KT, rows = min(KT, sample.keys - at);
+        load_tile<T, DP, KT, kThreads, Whole>(buffer_of(k + at * a.ks.token, rows, a.ks.token, a.dim), k_bytes, a.dim,
+                                              (LdsBytes) lds[tile & 1][0], threadIdx.x);
+        load_tile<T, DP, KT, kThreads, Whole>(buffer_of(v + at * a.vs.token, rows, a.vs.token, a.dim), v_bytes, a.dim,
+                                              (LdsBytes) lds[tile & 1][1], threadIdx.x);
+    };
+    if (tiles > 0)
+        load(0);
+
+    const bool there = i <= last;
+    const int64_t row = (static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + i;
+    Fragment<T, DP> q, d_o;
+    float delta, log2_sum = -kLowest;
+    {
+        Fragment<T, DP> o;
+        load_fragment<T, DP, Whole>(&o, a.o + n * a.os.sample + head * a.os.head + i * a.os.token, there, a.dim);
+        load_fragment<T, DP, Whole>(&d_o, a.d_o + n * a.d_os.sample + head * a.d_os.head + i * a.d_os.token, there, a.dim);
+        delta = dot<T, DP>(o, d_o);
+    }
+    load_fragment<T, DP, Whole>(&q, a.q + n * a.qs.sample + head * a.qs.head + i * a.qs.token, there, a.dim);
+    if (there)
+    {
+        const float l = a.logsumexp[row];
+        if (l > -INFINITY)
+            log2_sum = l * kLog2e;
+        if (lane < 32)
+        {
+            a.log2_sum[row] = log2_sum;
+            a.delta[row] = delta;
+        }
+    }
+    f32x16 dq[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+        dq[d] = zero16();
+    const int row_from = sample.first_key(min(i, max(last, 0))), row_end = sample.end_key(min(i, max(last, 0)));
+    const int some_from = sample.first_key(first), some_end = sample.end_key(last);
+    const int all_from = sample.first_key(last), all_end = sample.end_key(first);
+
+    for (int tile = 0; tile < tiles; ++tile)
+    {
+        wait_for_loads();
+        __syncthreads();
+        if (tile + 1 < tiles)
+            load(tile + 1);
+        const LdsBytes k_tile = (LdsBytes) lds[tile & 1][0], v_tile = (LdsBytes) lds[tile & 1][1];
+#pragma unroll
+        for (int b = 0; b < KT / 32; ++b)
+        {
+            const int at = from + tile * KT + 32 * b;
+            if (first > last || at >= some_end || at + 32 <= some_from)
+                continue;
+            f32x16 s = product<T, DP>(k_tile, 32 * b, q);
+            const f32x16 dp = product<T, DP>(v_tile, 32 * b, d_o);
+            if (at < all_from || at + 32 > all_end)
+                hide(&s, at, row_from, row_end);
+            Weights<T> ds;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+            {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale_log2, -log2_sum));
+                ds.set(j, p * (dp[j] - delta));
+            }
+            accumulate<DP>(k_tile, 32 * b, ds, dq);
+        }
+    }
+    if (i < a.masks.queries)
+        store_row<T, DP, Whole>(a.dq + n * a.dqs.sample + head * a.dqs.head + i * a.dqs.token, a.dim, dq, a.scale);
+#endif
+}
+
+// dk and dv: the waves of a workgroup take 32 keys of a key head each; the queries of the heads that share it pass through LDS, one head after
+// another.
+template <typename T, int DP, bool Whole>
+__global__ void __launch_bounds__(kThreads) attention_dkv_kernel(const Args<T> a)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    constexpr int QT = kTileRows<T>, kTileBytes = QT * Tile<T, DP>::kRowBytes;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
+    __shared__ __attribute__((aligned(16))) float stats[2][2][kWaveSize];
+    const uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
+    if (id >= a.total)
+        return;
+    const int key_heads = a.query_heads / a.group;
+    const int block = id % a.blocks; // (under a causal mask the first keys have the most queries)
+    const int key_head = id / a.blocks % key_heads, n = id / a.blocks / key_heads;
+    const int lane = threadIdx.x & (kWaveSize - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
+    const Sample sample = sample_of(a.masks, n);
+
+    const int block_first = block * (kWaves * kRows), block_end = min(block_first + kWaves * kRows, sample.keys);
+    const int first = block_first + wave * kRows, j = first + (lane & 31);
+    const int last = min(first + kRows, sample.keys) - 1;
+    int from = 0, tiles = 0;
+    if (block_first < block_end)
+    {
+        from = sample.first_query(block_first);
+        tiles = (max(sample.end_query(block_end - 1) - from, 0) + QT - 1) / QT;
+    }
+    const int q_bytes = static_cast<int>(a.qs.token * sizeof(T)), d_o_bytes = static_cast<int>(a.d_os.token * sizeof(T));
+    // tile `tile` of the group's head `g`, to stage `stage`
+    const auto load = [&](int g, int tile, int stage) {
+        const int head = key_head * a.group + g, at = from + tile * QT, rows = min(QT, sample.queries - at);
+        const T* const q = a.q + n * a.qs.sample + head * a.qs.head + at * a.qs.token;
+        const T* const d_o = a.d_o + n * a.d_os.sample + head * a.d_os.head + at * a.d_os.token;
+        load_tile<T, DP, QT, kThreads, Whole>(buffer_of(q, rows, a.qs.token, a.dim), q_bytes, a.dim, (LdsBytes) lds[stage][0],
+                                              threadIdx.x);
+        load_tile<T, DP, QT, kThreads, Whole>(buffer_of(d_o, rows, a.d_os.token, a.dim), d_o_bytes, a.dim, (LdsBytes) lds[stage][1],
+                                              threadIdx.x);
+        // rows' logarithms by one wave, their deltas by another (zero behind the sample's queries, as q and d_o are)
+        if (wave < 2)
+        {
+            const float* const p = (wave == 0 ? a.log2_sum : a.delta)
+                                   + (static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + at;
+            load_numbers(buffer_of(p, rows, 1, 1), (LdsBytes) stats[stage][wave], lane);
+        }
+    };
+    const int steps = tiles * a.group;
+    if (steps > 0)
+        load(0, 0, 0);
+
+    const bool there = j <= last;
+    Fragment<T, DP> k, v;
+    load_fragment<T, DP, Whole>(&k, a.k + n * a.ks.sample + key_head * a.ks.head + j * a.ks.token, there, a.dim);
+    load_fragment<T, DP, Whole>(&v, a.v + n * a.vs.sample + key_head * a.vs.head + j * a.vs.token, there, a.dim);
+    f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+        dk[d] = dv[d] = zero16();
+    const int row_from = sample.first_query(min(j, max(last, 0))), row_end = sample.end_query(min(j, max(last, 0)));
+    const int some_from = sample.first_query(first), some_end = sample.end_query(last);
+    const int all_from = sample.first_query(last), all_end = sample.end_query(first);
+
+    int g = 0, tile = 0;
+    for (int step = 0; step < steps; ++step)
+    {
+        const int stage = step & 1, here = from + tile * QT;
+        wait_for_loads();
+        __syncthreads();
+        if (++tile == tiles)
+            tile = 0, ++g;
+        if (step + 1 < steps)
+            load(g, tile, stage ^ 1);
+        const LdsBytes q_tile = (LdsBytes) lds[stage][0], d_o_tile = (LdsBytes) lds[stage][1];
+#pragma unroll
+        for (int b = 0; b < QT / 32; ++b)
+        {
+            const int at = here + 32 * b;
+            if (first > last || at >= some_end || at + 32 <= some_from)
+                continue;
+            f32x16 s = product<T, DP>(q_tile, 32 * b, k);
+            if (at < all_from || at + 32 > all_end)
+                hide(&s, at, row_from, row_end);
+            Weights<T> p, ds;
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+            {
+                const f32x4 l = *reinterpret_cast<const f32x4*>(&stats[stage][0][32 * b + 2 * r + 4 * (lane / 32)]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                {
+                    s[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + e], a.scale_log2, -l[e]));
+                    p.set(r + e, s[r + e]);
+                }
+            }
+            accumulate<DP>(d_o_tile, 32 * b, p, dv);
+            const f32x16 dp = product<T, DP>(d_o_tile, 32 * b, v);
+#pragma unroll
+            for (int r = 0; r < 16; r += 4)
+            {
+                const f32x4 delta = *reinterpret_cast<const f32x4*>(&stats[stage][1][32 * b + 2 * r + 4 * (lane / 32)]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    ds.set(r + e, s[r + e] * (dp[r + e] - delta[e]));
+            }
+            accumulate<DP>(q_tile, 32 * b, ds, dk);
+        }
+    }
+    if (j < a.masks.keys)
+    {
+        if (!there) // (a key of zeros may have had infinite weights)
+        {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+                dk[d] = dv[d] = zero16();
+        }
+        store_row<T, DP, Whole>(a.dk + n * a.dks.sample + key_head * a.dks.head + j * a.dks.token, a.dim, dk, a.scale);
+        store_row<T, DP, Whole>(a.dv + n * a.dvs.sample + key_head * a.dvs.head + j * a.dvs.token, a.dim, dv, 1.0f);
+    }
+#endif
+}
+
+// ---- host ------------------------------------------------------------------------------------------------------
+
+size_t rows_of(const h2x_attention& a)
+{
+    return static_cast<size_t>(a.samples) * a.query_heads * a.queries;
+}
+
+template <typename T, bool Whole>
+int issue(const h2x_attention& c, Args<T> a, hipStream_t stream)
+{
+    const int rows = kWaves * kRows;
+    const uint64_t query_blocks = (c.queries + rows - 1) / rows, key_blocks = (c.keys + rows - 1) / rows;
+    const uint64_t query_groups = query_blocks * c.samples * c.query_heads, key_groups = key_blocks * c.samples * c.key_heads;
+    if (query_groups > 0x800000u || key_groups > 0x800000u) // a grid of fewer than 2^32 threads
+        return H2X_ERR_TOO_LARGE;
+    const auto grid = [](uint64_t groups) { return dim3(static_cast<uint32_t>((groups + kNumXcd - 1) / kNumXcd * kNumXcd)); };
+    return with_padded_dim(c.head_dim, [&](auto dim) {
+        constexpr int DP = decltype(dim)::value;
+        if (query_groups > 0)
+        {
+            a.blocks = static_cast<int>(query_blocks);
+            a.total = static_cast<uint32_t>(query_groups);
+            launch(attention_dq_kernel<T, DP, Whole>, grid(query_groups), dim3(kThreads), stream, a);
+        }
+        if (key_groups > 0)
+        {
+            a.blocks = static_cast<int>(key_blocks);
+            a.total = static_cast<uint32_t>(key_groups);
+            launch(attention_dkv_kernel<T, DP, Whole>, grid(key_groups), dim3(kThreads), stream, a);
+        }
+        return launch_status();
+    });
+}
+
+} // namespace
+} // namespace attention
+} // namespace h2x
+
+using namespace h2x;
+using namespace h2x::attention;
+
+extern "C" size_t h2x_attention_backward_workspace_bytes(const h2x_attention* attention)
+{
+    return check(attention) == H2X_SUCCESS ? 8 * rows_of(*attention) : 0;
+}
+
+extern "C" int h2x_attention_backward(const h2x_attention* attention, const void* q, const void* k, const void* v, const void* o,
+                                      const void* d_o, const float* logsumexp, const int32_t* query_lengths,
+                                      const int32_t* key_lengths, void* dq, void* dk, void* dv, void* workspace,
+                                      h2x_stream_t stream)
+{
+    if (const int bad = check(attention))
+        return bad;
+    const h2x_attention& c = *attention;
+    struct Operand
+    {
+        const void* p;
+        const h2x_token_strides* given;
+        int64_t tokens;
+        int heads;
+        bool output;
+        Strides s;
+    } operands[] = {{q, &c.q, c.queries, c.query_heads, false},     {k, &c.k, c.keys, c.key_heads, false},
+                    {v, &c.v, c.keys, c.key_heads, false},          {o, &c.o, c.queries, c.query_heads, false},
+                    {d_o, &c.d_o, c.queries, c.query_heads, false}, {dq, &c.dq, c.queries, c.query_heads, true},
+                    {dk, &c.dk, c.keys, c.key_heads, true},         {dv, &c.dv, c.keys, c.key_heads, true}};
+    bool whole = true, missing = false;
+    for (Operand& x : operands)
+    {
+        x.s = strides_of(c, *x.given, x.tokens, x.heads);
+        if (const int bad = check_strides(c, x.s, x.tokens, x.heads, x.output))
+            return bad;
+        whole = whole && whole_rows(c, x.p, x.s);
+        missing = missing || (!x.p && x.tokens > 0);
+    }
+    if (c.samples == 0 || c.query_heads == 0 || (c.queries == 0 && c.keys == 0))
+        return H2X_SUCCESS;
+    if (missing || (c.queries > 0 && (!logsumexp || !workspace)))
+        return H2X_ERR_INVALID_ARGUMENT;
+    return with_elements(c.dtype, whole, [&](auto t, auto is_whole) {
+        using T = decltype(t);
+        Args<T> a{};
+        a.q = static_cast<const T*>(q);
+        a.k = static_cast<const T*>(k);
+        a.v = static_cast<const T*>(v);
+        a.o = static_cast<const T*>(o);
+        a.d_o = static_cast<const T*>(d_o);
+        a.logsumexp = logsumexp;
+        a.dq = static_cast<T*>(dq);
+        a.dk = static_cast<T*>(dk);
+        a.dv = static_cast<T*>(dv);
+        a.log2_sum = static_cast<float*>(workspace);
+        a.delta = a.log2_sum + rows_of(c);
+        Strides* const strides[] = {&a.qs, &a.ks, &a.vs, &a.os, &a.d_os, &a.dqs, &a.dks, &a.dvs};
+        for (int i = 0; i < 8; ++i)
+            *strides[i] = operands[i].s;
+        a.masks = masks_of(c, query_lengths, key_lengths);
+        a.scale = static_cast<float>(c.scale);
+        a.scale_log2 = static_cast<float>(c.scale * 1.4426950408889634);
+        a.dim = c.head_dim;
+        a.query_heads = c.query_heads;
+        a.group = c.query_heads / c.key_heads;
+        return issue<T, decltype(is_whole)::value>(c, a, as_stream(stream));
+    });
+}

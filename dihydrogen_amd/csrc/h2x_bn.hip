@@ -3928,6 +3928,7 @@ using namespace h2x;
     {                                                                                              \
     case H2X_F32: return CALL_F32;                                                                 \
     case H2X_F64: return CALL_F64;                                                                 \
+    default: break;                                                                                \
     }                                                                                              \
     return H2X_ERR_UNSUPPORTED
 

@@ -363,6 +363,14 @@ PyMethodDef s_methods[] = {H2X_ENTRY(h2x_bn_channel_sums_and_sqsums),
                            H2X_ENTRY(h2x_shuffle_direct),
                            H2X_ENTRY(h2x_shuffle_pack_batched),
                            H2X_ENTRY(h2x_shuffle_unpack_batched),
+                           H2X_ENTRY(h2x_layer_norm_forward),
+                           H2X_ENTRY(h2x_layer_norm_workspace_bytes),
+                           H2X_ENTRY(h2x_layer_norm_backward),
+                           H2X_ENTRY(h2x_rotary_apply),
+                           H2X_ENTRY(h2x_attention_forward_workspace_bytes),
+                           H2X_ENTRY(h2x_attention_forward),
+                           H2X_ENTRY(h2x_attention_backward_workspace_bytes),
+                           H2X_ENTRY(h2x_attention_backward),
                            {"pointer_types",
                             reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&pointer_types)), METH_FASTCALL, nullptr},
                            {"same_buffers",

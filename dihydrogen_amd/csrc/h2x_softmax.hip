@@ -2291,6 +2291,7 @@ extern "C" int h2x_softmax_channel_forward(h2x_dtype dtype, int num_samples, int
         return forward_impl<float>(num_samples, num_channels, spatial_size, x, y, as_stream(stream));
     case H2X_F64:
         return forward_impl<double>(num_samples, num_channels, spatial_size, x, y, as_stream(stream));
+    default: break;
     }
     return H2X_ERR_UNSUPPORTED;
 }
@@ -2313,6 +2314,7 @@ extern "C" int h2x_softmax_channel_backward(h2x_dtype dtype, int num_samples, in
         return backward_impl<float>(num_samples, num_channels, spatial_size, y, dy, dx, as_stream(stream));
     case H2X_F64:
         return backward_impl<double>(num_samples, num_channels, spatial_size, y, dy, dx, as_stream(stream));
+    default: break;
     }
     return H2X_ERR_UNSUPPORTED;
 }
@@ -2334,6 +2336,7 @@ extern "C" size_t h2x_softmax_instance_workspace_bytes(int num_samples)
     {                                                                                              \
     case H2X_F32: return CALL_F32;                                                                 \
     case H2X_F64: return CALL_F64;                                                                 \
+    default: break;                                                                                \
     }                                                                                              \
     return H2X_ERR_UNSUPPORTED
 

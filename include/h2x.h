@@ -2,7 +2,9 @@
  * h2x.h -- C ABI of the MI355X (gfx950) implementation of DistConv's
  * data-parallel, non-convolution hot path: channel-wise batch-norm statistics
  * (forward and backward), halo pack/unpack of spatially decomposed tensors,
- * channel softmax (forward and backward) and the tensor-shuffler pack/unpack.
+ * channel softmax (forward and backward) and the tensor-shuffler pack/unpack;
+ * and of what such a network needs where it treats the cells of its grid as
+ * tokens: layer normalisation, rotary positions and attention.
  *
  * Every entry point takes plain device pointers, sizes and a HIP stream, is
  * asynchronous on that stream, performs no device synchronisation and no
@@ -43,11 +45,16 @@ typedef enum h2x_status
     H2X_ERR_SCRATCH_LIMIT = -4 /* beyond the fixed capacity of an entry point that allocates nothing */
 } h2x_status;
 
-/** Element type of floating-point tensors (batch-norm, softmax, halo accumulate). */
+/**
+ * Element type of floating-point tensors.  Batch-norm, softmax, halo accumulate
+ * and the transforms take H2X_F32 and H2X_F64; the token operators say which they take.
+ */
 typedef enum h2x_dtype
 {
     H2X_F32 = 0,
-    H2X_F64 = 1
+    H2X_F64 = 1,
+    H2X_BF16 = 2,
+    H2X_F16 = 3
 } h2x_dtype;
 
 /** legacy/include/distconv/base.hpp:23 */
@@ -1302,6 +1309,188 @@ int h2x_shuffle_direct_plan_destroy(h2x_shuffle_direct_plan* plan);
  */
 int h2x_shuffle_direct(const h2x_shuffle_direct_plan* plan, void* const* src, void* const* dst, int backward,
                        h2x_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Token operators: layer normalisation, rotary positions, attention         */
+/*                                                                           */
+/* A token is a cell of the (local) grid; its channels, or the elements of   */
+/* its heads, lie innermost in memory, one element apart.  These have no     */
+/* counterpart in the reference.                                             */
+/* ------------------------------------------------------------------------ */
+
+/**
+ * Layer normalisation of `num_rows` rows of `num_channels` elements, each on its own:
+ *   mean = sum x / C;  rstd = 1 / sqrt(sum (x - mean)^2 / C + epsilon);
+ *   y = (x - mean) * rstd * scale + bias.
+ * dtype: any h2x_dtype; scale, bias: weight_dtype, which is dtype or H2X_F32 (H2X_F64 with H2X_F64 only);
+ * either may be NULL (1 and 0).  mean, rstd: num_rows elements, float (double with H2X_F64), what the
+ * backward pass needs; both or neither may be NULL.
+ *
+ * x_rows, y_rows: NULL where row r starts at r * num_channels; otherwise the rows of a tensor
+ * of 1 to H2X_MAX_DIMS dimensions with local_shape[0] == num_channels, strides[0] == 1 and num_rows as
+ * the product of the other extents, r counting through them innermost first (the interior of a
+ * haloed tensor whose channel is innermost).  y may be x itself, with the same rows.  Sums are in 32 bits (64
+ * with H2X_F64), the squares' about the mean.  num_rows up to 2^31 - 1.
+ */
+int h2x_layer_norm_forward(h2x_dtype dtype,
+                           h2x_dtype weight_dtype,
+                           size_t num_rows,
+                           int num_channels,
+                           const h2x_tensor_geometry* x_rows,
+                           const h2x_tensor_geometry* y_rows,
+                           const void* x,
+                           const void* scale,
+                           const void* bias,
+                           void* y,
+                           void* mean,
+                           void* rstd,
+                           double epsilon,
+                           h2x_stream_t stream);
+
+/** Bytes of workspace for h2x_layer_norm_backward with gradients of scale or bias: no initialisation, no state
+ * between calls; not for two calls that may run at the same time. */
+size_t h2x_layer_norm_workspace_bytes(h2x_dtype dtype, size_t num_rows, int num_channels);
+
+/**
+ * Gradients, with h = (x - mean) * rstd and g = dy * scale:
+ *   dx = rstd * (g - sum g / C - h * sum (g h) / C);  dscale = sum over rows of dy * h;  dbias = sum over rows of dy.
+ * mean, rstd: of the forward pass.  dscale, dbias: weight_dtype, overwritten (zero without rows); either may be NULL,
+ * workspace too where both are.  dx may be NULL, or x or dy itself with the same rows.  Sums over rows are made in
+ * a fixed order: in 32 bits over the rows of a workgroup and in 64 over workgroups.
+ */
+int h2x_layer_norm_backward(h2x_dtype dtype,
+                            h2x_dtype weight_dtype,
+                            size_t num_rows,
+                            int num_channels,
+                            const h2x_tensor_geometry* x_rows,
+                            const h2x_tensor_geometry* dy_rows,
+                            const h2x_tensor_geometry* dx_rows,
+                            const void* x,
+                            const void* dy,
+                            const void* mean,
+                            const void* rstd,
+                            const void* scale,
+                            void* dx,
+                            void* dscale,
+                            void* dbias,
+                            void* workspace,
+                            h2x_stream_t stream);
+
+/** Where element (sample, token, head, i) of a tensor lies: base[sample * sample_stride + token * token_stride +
+ * head * head_stride + i], strides in elements. */
+typedef struct h2x_token_strides
+{
+    int64_t sample, token, head;
+} h2x_token_strides;
+
+#define H2X_MAX_AXES 4
+
+/** How the elements of a head are paired, with m pairs in all: (i, i + m) or (2 i, 2 i + 1). */
+typedef enum h2x_rotary_pairing
+{
+    H2X_ROTARY_HALVES = 0,
+    H2X_ROTARY_NEIGHBOURS = 1
+} h2x_rotary_pairing;
+
+/**
+ * Rotary positions with several axes: pair i belongs to an axis a, the first axis_pairs[0] pairs to axis 0, the next
+ * axis_pairs[1] to axis 1 and so on, and is turned by the angle positions[a] * frequencies[i]:
+ *   (u, v) -> (u cos - v sin, u sin + v cos).
+ * Elements behind the 2 * sum(axis_pairs) that are paired are copied.
+ */
+typedef struct h2x_rotary
+{
+    int32_t dtype; /* any h2x_dtype */
+    int32_t pairing;
+    int32_t head_dim, heads, samples, num_axes;
+    int64_t tokens;
+    int32_t axis_pairs[H2X_MAX_AXES];
+    /* element (sample, axis, token) of positions lies at sample * positions_sample_stride + axis * positions_axis_stride +
+     * token; a sample stride of 0: all samples have the same */
+    int64_t positions_sample_stride, positions_axis_stride;
+    h2x_token_strides x, y;
+} h2x_rotary;
+
+/**
+ * Turns the heads of x by their positions into y; inverse != 0: by minus the angles, which is the gradient of the turn.
+ * positions: int32 on the device.  frequencies: doubles on the device, one for each pair, radians a step.  Angles are made
+ * in 64 bits, at positions of 31 bits too.  y may be x itself, with the same strides.
+ */
+int h2x_rotary_apply(const h2x_rotary* rotary,
+                     const void* x,
+                     const int32_t* positions,
+                     const double* frequencies,
+                     int inverse,
+                     void* y,
+                     h2x_stream_t stream);
+
+/**
+ * Attention of `queries` tokens to `keys` tokens in each sample, head by head; query head h uses key head
+ * h / (query_heads / key_heads).
+ *
+ * Lengths: sample b has query_lengths[b] queries and key_lengths[b] keys (int32 on the device; NULL: all have `queries` and `keys`;
+ * values are clamped to 0 and these).  What lies behind a sample's lengths is not used, whatever its values.
+ * Mask: the last query of a sample stands at its last key, so query i stands at place(i) = i + its keys - its queries, and sees the keys
+ * j with place(i) - window_left <= j <= place(i) + window_right; a negative window_left or window_right has no bound
+ * (window_right = 0: a query sees no key behind its own place).  Keys and values within a sample's lengths have to be finite.
+ * Empty rows (a query that sees no key, or lies behind its sample's queries) have output zero and a logarithm of minus infinity, and give
+ * no gradients; rows of the gradients behind the lengths are zero.
+ */
+typedef struct h2x_attention
+{
+    int32_t dtype;    /* H2X_BF16 or H2X_F32 */
+    int32_t head_dim; /* 1 to 128 */
+    int32_t samples, query_heads, key_heads, reserved;
+    int64_t queries, keys; /* below 2^31 */
+    int64_t window_left, window_right;
+    double scale;
+    h2x_token_strides q, k, v, o;         /* token strides of at least head_dim elements */
+    h2x_token_strides d_o, dq, dk, dv;    /* the backward pass alone */
+} h2x_attention;
+
+/** Bytes of workspace of h2x_attention_forward (0: none), without initialisation or state between calls; not for two calls that may
+ * run at the same time. */
+size_t h2x_attention_forward_workspace_bytes(const h2x_attention* attention);
+
+/**
+ * s = scale * q k^T;  p = exp(s - logsumexp) where a query sees a key;  o = p v;  logsumexp = log sum exp s, in 32 bits, at
+ * (sample * query_heads + head) * queries + query, or NULL.  Scores, sums and outputs are accumulated in 32 bits; with
+ * H2X_BF16 the probabilities are rounded to 16 bits for the product with v.
+ */
+int h2x_attention_forward(const h2x_attention* attention,
+                          const void* q,
+                          const void* k,
+                          const void* v,
+                          const int32_t* query_lengths,
+                          const int32_t* key_lengths,
+                          void* o,
+                          float* logsumexp,
+                          void* workspace,
+                          h2x_stream_t stream);
+
+/** The same for h2x_attention_backward. */
+size_t h2x_attention_backward_workspace_bytes(const h2x_attention* attention);
+
+/**
+ * Gradients, recomputing p from logsumexp; with delta = sum over a head's elements of d_o * o:
+ *   dv = p^T d_o;  ds = p (d_o v^T - delta);  dq = scale * ds k;  dk = scale * ds^T q;
+ * dk and dv of a key head are sums over the query heads that share it.  o, logsumexp: of the forward pass.  Every sum is
+ * made in a fixed order.  Outputs may not overlap inputs.
+ */
+int h2x_attention_backward(const h2x_attention* attention,
+                           const void* q,
+                           const void* k,
+                           const void* v,
+                           const void* o,
+                           const void* d_o,
+                           const float* logsumexp,
+                           const int32_t* query_lengths,
+                           const int32_t* key_lengths,
+                           void* dq,
+                           void* dk,
+                           void* dv,
+                           void* workspace,
+                           h2x_stream_t stream);
 
 #ifdef __cplusplus
 }
