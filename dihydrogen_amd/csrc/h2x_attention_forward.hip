@@ -379,41 +379,53 @@ __global__ void __launch_bounds__(kThreads) attention_few_kernel(const Args<T> a
 #endif
 }
 
-// Joins the parts of a row, a wave a row.
+// Joins the parts of a row, a workgroup a row: a lane has a part's maximum and sum, a wave every fourth part's output.  (With a wave a row, one
+// part after another, 512 rows of 16 parts took 21 us: a chain of waits for memory.)
+constexpr int kMostParts = kWaveSize;
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(const Args<T> a)
 {
-    const int64_t rows = static_cast<int64_t>(a.samples) * a.query_heads * a.masks.queries;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWaves + threadIdx.x / kWaveSize;
-    const int lane = threadIdx.x & (kWaveSize - 1);
-    if (row >= rows)
-        return;
-    float max = kLowest;
-    for (int p = 0; p < a.parts.num; ++p)
-        max = fmaxf(max, a.parts.max_sum[2 * (p * rows + row)]);
-    float sum = 0.0f, out[(DP + kWaveSize - 1) / kWaveSize] = {};
-    for (int p = 0; p < a.parts.num; ++p)
+    constexpr int N = (DP + kWaveSize - 1) / kWaveSize; // elements of a lane
+    __shared__ float outs[kWaves][N * kWaveSize], factors[kMostParts];
+    const int64_t rows = static_cast<int64_t>(a.samples) * a.query_heads * a.masks.queries, row = blockIdx.x;
+    const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
+    float max = kLowest, sum = 0.0f;
+    if (lane < a.parts.num)
     {
-        const float share = a.parts.max_sum[2 * (p * rows + row) + 1];
-        if (!(share > 0.0f)) // no key of the part: its output was not written
-            continue;
-        const float factor = exp2f(a.parts.max_sum[2 * (p * rows + row)] - max);
-        sum = __builtin_fmaf(share, factor, sum);
-#pragma unroll
-        for (int d = 0; d < DP; d += kWaveSize)
-            if (d + lane < DP)
-                out[d / kWaveSize] = __builtin_fmaf(a.parts.out[(p * rows + row) * DP + d + lane], factor, out[d / kWaveSize]);
+        max = a.parts.max_sum[2 * (lane * rows + row)];
+        sum = a.parts.max_sum[2 * (lane * rows + row) + 1];
     }
+    const bool any = sum > 0.0f; // (where no key was seen the output was not written)
+    const float most = wave_combine(any ? max : kLowest, [](float x, float y) { return fmaxf(x, y); });
+    const float factor = any ? __builtin_amdgcn_exp2f(max - most) : 0.0f;
+    if (wave == 0)
+        factors[lane] = factor;
+    sum = token::wave_total(sum * factor);
+    __syncthreads();
+    float out[N] = {};
+#pragma unroll 4
+    for (int p = wave; p < a.parts.num; p += kWaves)
+    {
+        const float f = factors[p];
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+        {
+            const float x = n * kWaveSize + lane < DP ? a.parts.out[(p * rows + row) * DP + n * kWaveSize + lane] : 0.0f;
+            out[n] = f > 0.0f ? __builtin_fmaf(x, f, out[n]) : out[n];
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+        outs[wave][n * kWaveSize + lane] = out[n];
+    __syncthreads();
+    const int d = threadIdx.x;
     const int64_t of_head = row / a.masks.queries, i = row - of_head * a.masks.queries;
     const int64_t n = of_head / a.query_heads, head = of_head - n * a.query_heads;
     T* const o = a.o + n * a.os.sample + head * a.os.head + i * a.os.token;
-    const float scale = sum > 0.0f ? 1.0f / sum : 0.0f;
-#pragma unroll
-    for (int d = 0; d < DP; d += kWaveSize)
-        if (d + lane < a.dim)
-            o[d + lane] = static_cast<T>(out[d / kWaveSize] * scale);
-    if (a.logsumexp && lane == 0)
-        a.logsumexp[row] = sum > 0.0f ? (max + log2f(sum)) * kLn2 : -INFINITY;
+    if (d < a.dim)
+        o[d] = static_cast<T>(sum > 0.0f ? (outs[0][d] + outs[1][d] + outs[2][d] + outs[3][d]) / sum : 0.0f);
+    if (a.logsumexp && d == 0)
+        a.logsumexp[row] = sum > 0.0f ? (most + log2f(sum)) * kLn2 : -INFINITY;
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------
@@ -439,7 +451,7 @@ Plan plan_of(const h2x_attention& a)
     const int tile = a.dtype == H2X_F32 ? 32 : 64;
     const int64_t least = p.few ? 4 * kWaves * tile : 8 * tile, aim = (p.few ? 8 : 2) * static_cast<int64_t>(chip_units());
     int64_t parts = 1;
-    while (parts < 64 && groups * parts < aim && a.keys >= 2 * parts * least)
+    while (parts < kMostParts && groups * parts < aim && a.keys >= 2 * parts * least)
         parts *= 2;
     p.query_blocks = static_cast<int>(blocks);
     p.parts = static_cast<int>(parts);
@@ -469,8 +481,7 @@ int issue(const h2x_attention& c, const Plan& p, const Args<T>& a, hipStream_t s
         else
             launch(attention_forward_kernel<T, DP, Whole>, grid, dim3(kThreads), stream, a);
         if (p.parts > 1)
-            launch(attention_join_kernel<T, DP>, dim3(static_cast<uint32_t>((rows_of(c) + kWaves - 1) / kWaves)), dim3(kThreads),
-                   stream, a);
+            launch(attention_join_kernel<T, DP>, dim3(static_cast<uint32_t>(rows_of(c))), dim3(kThreads), stream, a);
         return launch_status();
     });
 }
@@ -508,7 +519,7 @@ extern "C" int h2x_attention_forward(const h2x_attention* attention, const void*
     const Plan p = plan_of(c);
     if (!q || !o || (c.keys > 0 && (!k || !v)) || (p.parts > 1 && !workspace))
         return H2X_ERR_INVALID_ARGUMENT;
-    if (p.groups > 0x800000u || (p.parts > 1 && rows_of(c) > 0x2000000u))
+    if (p.groups > 0x800000u || (p.parts > 1 && rows_of(c) > 0x800000u))
         return H2X_ERR_TOO_LARGE; // (a grid of fewer than 2^32 threads)
     const bool whole = whole_rows(c, q, qs) && whole_rows(c, k, ks) && whole_rows(c, v, vs) && whole_rows(c, o, os);
     return with_elements(c.dtype, whole, [&](auto t, auto is_whole) {

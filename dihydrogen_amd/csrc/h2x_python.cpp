@@ -312,6 +312,45 @@ PyObject* same_buffers(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     return PyBool_FromLong(k == n);
 }
 
+// layout_key(number, *tensors): bytes that are equal for equal numbers and tensors alike in type, device, extents and strides, None's
+// among them; None where torch tensors are not known, or something else is among the arguments. (With `shape`,
+// `stride()` and so on from Python the key of a normalisation took 3 us, longer than its launch.)
+PyObject* layout_key(PyObject*, PyObject* const* args, Py_ssize_t nargs)
+{
+    constexpr Py_ssize_t kMost = 512;
+    int64_t key[kMost];
+    Py_ssize_t n = 0;
+    if (nargs < 1 || !s_torch_is_known)
+        Py_RETURN_NONE;
+    key[n++] = PyLong_AsLongLong(args[0]);
+    if (key[0] == -1 && PyErr_Occurred())
+        return nullptr;
+    for (Py_ssize_t a = 1; a < nargs; ++a)
+    {
+        if (args[a] == Py_None)
+        {
+            if (n == kMost)
+                Py_RETURN_NONE;
+            key[n++] = -1;
+            continue;
+        }
+        if (!PyObject_TypeCheck(args[a], s_torch_tensor))
+            Py_RETURN_NONE;
+        const at::Tensor& t = THPVariable_Unpack(args[a]);
+        if (!t.defined() || t.layout() != at::kStrided || t.unsafeGetTensorImpl()->has_symbolic_sizes_strides()
+            || n + 1 + 2 * t.dim() > kMost)
+            Py_RETURN_NONE;
+        key[n++] = t.dim() << 32 | static_cast<int64_t>(t.scalar_type()) << 16 | static_cast<int64_t>(t.device().type()) << 8
+                   | (t.device().index() & 0xff);
+        for (int64_t d = 0; d < t.dim(); ++d)
+        {
+            key[n++] = t.size(d);
+            key[n++] = t.stride(d);
+        }
+    }
+    return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(key), n * sizeof(int64_t));
+}
+
 #define H2X_ENTRY(NAME)                                                                            \
     {                                                                                              \
         #NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&Entry<NAME>::fastcall)), \
@@ -373,6 +412,8 @@ PyMethodDef s_methods[] = {H2X_ENTRY(h2x_bn_channel_sums_and_sqsums),
                            H2X_ENTRY(h2x_attention_backward),
                            {"pointer_types",
                             reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&pointer_types)), METH_FASTCALL, nullptr},
+                           {"layout_key",
+                            reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&layout_key)), METH_FASTCALL, nullptr},
                            {"same_buffers",
                             reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&same_buffers)), METH_FASTCALL, nullptr},
                            {nullptr, nullptr, 0, nullptr}};

@@ -29,9 +29,22 @@ def _require(condition: bool, what: str) -> None:
         raise ValueError(what)
 
 
-def _on_one_gpu(stream: Optional[torch.cuda.Stream], *tensors: Optional[torch.Tensor]) -> None:
+def _current_device() -> int:
+    return torch._C._cuda_getDevice() if _initialized() else _first_device()
+
+
+_initialized = torch.cuda.is_initialized
+
+
+def _first_device() -> int:
+    if not torch.cuda.is_available():
+        return -1
+    torch.cuda.init()
+    return torch._C._cuda_getDevice()
+
+
+def _on_one_gpu(device: int, stream: Optional[torch.cuda.Stream], *tensors: Optional[torch.Tensor]) -> None:
     """All tensors are on the current GPU, to which the launches go, and the layer's stream too."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else None
     if stream is not None and stream.device_index != device:
         raise ValueError(f"the layer's stream is on GPU {stream.device_index}, the current one is {device}")
     for t in tensors:
@@ -40,13 +53,21 @@ def _on_one_gpu(stream: Optional[torch.cuda.Stream], *tensors: Optional[torch.Te
 
 
 class _Plans(dict):
-    """What is worked out for tensors of given shapes and strides, a bounded number of them."""
+    """What is worked out for tensors of given types, devices, extents and strides, for a bounded number of them."""
 
     def keep(self, key, plan):
         if len(self) >= 256:
             self.clear()
         self[key] = plan
         return plan
+
+
+def _key(calls, device: int, *tensors: Optional[torch.Tensor]):
+    """Equal for tensors alike, on the same current device."""
+    key = calls.layout_key(device, *tensors)
+    if key is None:
+        key = (device, *((t.dtype, t.device, t.shape, t.stride()) if t is not None else None for t in tensors))
+    return key
 
 
 def _view(t):
@@ -86,13 +107,8 @@ class LayerNormalization:
         self._calls = capi.calls()
         self._plans = _Plans()
 
-    def _plan(self, weights: Tuple, saved: Tuple, x: torch.Tensor, *others: torch.Tensor):
-        """Types, sizes and where rows lie, checked; worked out once for tensors alike."""
-        key = (x.dtype, x.shape, x.stride(), *((t.dtype, t.shape, t.stride()) for t in others),
-               *((t.dtype, t.shape, t.is_contiguous()) if t is not None else None for t in (*weights, *saved)))
-        plan = self._plans.get(key)
-        if plan is not None:
-            return plan
+    def _plan(self, key, device: int, weights: Tuple, saved: Tuple, x: torch.Tensor, *others: torch.Tensor):
+        """Types, sizes and where rows lie, checked."""
         dtype = _DTYPES.get(x.dtype)
         _require(dtype is not None, f"layer normalisation of {x.dtype} elements is not supported")
         _require(x.dim() >= 1 and x.shape[-1] >= 1, "rows of one element at least")
@@ -107,19 +123,20 @@ class LayerNormalization:
             _require(w.dtype == weight_dtype and w.shape == (channels,) and w.is_contiguous(),
                      "scale, bias and their gradients: one contiguous element of one type a channel")
         kept = torch.float64 if x.dtype == torch.float64 else torch.float32
+        _require(len([s for s in saved if s is None]) in (0, len(saved)), "mean and rstd go together")
         for s in saved:
             _require(s is None or (s.dtype == kept and s.numel() == rows and s.is_contiguous()),
                      f"mean and rstd: one contiguous {kept} a row")
         geometries = [_rows(t) for t in (x, *others)]
-        return self._plans.keep(key, (dtype, _DTYPES[weight_dtype], rows, channels, geometries,
-                                      [_address(g) for g in geometries]))
+        _on_one_gpu(device, self.stream, x, *others, *weights, *saved)
+        return self._plans.keep(key, (dtype, _DTYPES[weight_dtype], rows, channels, [_address(g) for g in geometries], geometries))
 
     def forward(self, input, scale: Optional[torch.Tensor], bias: Optional[torch.Tensor], output,
                 mean: Optional[torch.Tensor] = None, rstd: Optional[torch.Tensor] = None) -> int:
-        x, y = _view(input), _view(output)
-        _require((mean is None) == (rstd is None), "mean and rstd go together")
-        dtype, weight_dtype, rows, channels, _, (xg, yg) = self._plan((scale, bias), (mean, rstd), x, y)
-        _on_one_gpu(self.stream, x, y, scale, bias, mean, rstd)
+        x, y, device = _view(input), _view(output), _current_device()
+        key = _key(self._calls, device, x, y, scale, bias, mean, rstd)
+        plan = self._plans.get(key) or self._plan(key, device, (scale, bias), (mean, rstd), x, y)
+        dtype, weight_dtype, rows, channels, (xg, yg), _ = plan
         status = self._calls.h2x_layer_norm_forward(dtype, weight_dtype, rows, channels, xg, yg, x, scale, bias, y, mean, rstd,
                                                     self.epsilon, _stream_handle(self.stream))
         if status:
@@ -129,11 +146,13 @@ class LayerNormalization:
     def backward(self, input, d_output, mean: torch.Tensor, rstd: torch.Tensor, scale: Optional[torch.Tensor], d_input,
                  scale_gradient: Optional[torch.Tensor] = None, bias_gradient: Optional[torch.Tensor] = None) -> int:
         """Gradients; d_input may be input or d_output itself.  Gradients of scale and bias are overwritten."""
-        x, dy, dx = _view(input), _view(d_output), _view(d_input)
-        dtype, weight_dtype, rows, channels, _, (xg, dyg, dxg) = self._plan(
-            (scale, scale_gradient, bias_gradient), (mean, rstd), x, dy, dx)
-        _require(mean is not None and rstd is not None, "the backward pass needs mean and rstd")
-        _on_one_gpu(self.stream, x, dy, dx, mean, rstd, scale, scale_gradient, bias_gradient)
+        x, dy, dx, device = _view(input), _view(d_output), _view(d_input), _current_device()
+        key = _key(self._calls, device, x, dy, dx, mean, rstd, scale, scale_gradient, bias_gradient)
+        plan = self._plans.get(key)
+        if plan is None:
+            _require(mean is not None and rstd is not None, "the backward pass needs mean and rstd")
+            plan = self._plan(key, device, (scale, scale_gradient, bias_gradient), (mean, rstd), x, dy, dx)
+        dtype, weight_dtype, rows, channels, (xg, dyg, dxg), _ = plan
         ws = None
         if scale_gradient is not None or bias_gradient is not None:
             ws = _buffer_of(self.stream, self._calls.h2x_layer_norm_workspace_bytes(dtype, rows, channels), torch.uint8)
@@ -200,11 +219,7 @@ class RotaryPositions:
             torch.cuda.current_stream(device).synchronize()  # whatever stream comes next finds them
         return kept
 
-    def _plan(self, x: torch.Tensor, positions: torch.Tensor, y: torch.Tensor):
-        key = (x.dtype, x.shape, x.stride(), y.dtype, y.shape, y.stride(), positions.dtype, positions.shape, positions.stride())
-        plan = self._plans.get(key)
-        if plan is not None:
-            return plan
+    def _plan(self, key, device: int, x: torch.Tensor, positions: torch.Tensor, y: torch.Tensor):
         _require(x.dtype in _DTYPES, f"rotary positions of {x.dtype} elements are not supported")
         _require(_is_token_tensor(x) and _is_token_tensor(y), "(samples, tokens, heads, elements), the elements contiguous")
         _require(x.shape == y.shape and x.dtype == y.dtype, "tensors of one shape and type")
@@ -221,15 +236,16 @@ class RotaryPositions:
         r.positions_sample_stride = positions.stride(0) if positions.dim() == 3 else 0
         r.positions_axis_stride = positions.stride(-2)
         r.x, r.y = _token_strides(x), _token_strides(y)
-        return self._plans.keep(key, (r, ctypes.addressof(r)))
+        _on_one_gpu(device, self.stream, x, positions, y)
+        return self._plans.keep(key, (ctypes.addressof(r), x.stride() == y.stride(), r, self._frequencies(x.device)))
 
     def _apply(self, x: torch.Tensor, positions: torch.Tensor, y: torch.Tensor, inverse: int) -> int:
-        plan, address = self._plan(x, positions, y)
-        _on_one_gpu(self.stream, x, positions, y)
-        if x.data_ptr() == y.data_ptr():
-            _require(x.stride() == y.stride(), "in place: the same strides")
-        status = self._calls.h2x_rotary_apply(address, x, positions, self._frequencies(x.device), inverse, y,
-                                              _stream_handle(self.stream))
+        device = _current_device()
+        key = _key(self._calls, device, x, positions, y)
+        address, alike, _, frequencies = self._plans.get(key) or self._plan(key, device, x, positions, y)
+        if not alike:
+            _require(x.data_ptr() != y.data_ptr(), "in place: the same strides")
+        status = self._calls.h2x_rotary_apply(address, x, positions, frequencies, inverse, y, _stream_handle(self.stream))
         if status:
             capi.check(status, "rotary positions")
         return 0
@@ -265,18 +281,21 @@ class Attention:
         if causal:
             _require(right in (None, 0), "a causal window has no keys behind a query's place")
             right = 0
-        self.scale, self.window, self.stream = scale, (left, right), stream
+        self._scale, self._window, self.stream = scale, (left, right), stream  # (fixed: plans are made with them)
         self._calls = capi.calls()
         self._plans = _Plans()
 
-    def _plan(self, q, k, v, o, lse, lengths, gradients=()):
-        """h2x_attention for these tensors, checked; worked out once for tensors alike."""
+    @property
+    def scale(self) -> Optional[float]:
+        return self._scale
+
+    @property
+    def window(self) -> Tuple[Optional[int], Optional[int]]:
+        return self._window
+
+    def _plan(self, key, device: int, q, k, v, o, lse, lengths, gradients=()):
+        """h2x_attention for these tensors, checked."""
         tensors = (q, k, v, o, *gradients)
-        key = (self.scale, self.window, *((t.dtype, t.shape, t.stride()) for t in tensors),
-               *((t.dtype, t.shape, t.is_contiguous()) if t is not None else None for t in (lse, *lengths)))
-        plan = self._plans.get(key)
-        if plan is not None:
-            return plan
         _require(q.dtype in (torch.bfloat16, torch.float32), f"attention of {q.dtype} elements is not supported")
         _require(all(_is_token_tensor(t) and t.dtype == q.dtype for t in tensors),
                  "(samples, tokens, heads, elements) of one type, the elements contiguous")
@@ -295,21 +314,24 @@ class Attention:
         a = capi.Attention()
         a.dtype, a.head_dim, a.samples, a.query_heads, a.key_heads, a.queries, a.keys = (
             _DTYPES[q.dtype], dim, n, heads, key_heads, queries, keys)
-        a.window_left, a.window_right = (-1 if w is None else w for w in self.window)
-        a.scale = dim ** -0.5 if self.scale is None else self.scale
+        a.window_left, a.window_right = (-1 if w is None else w for w in self._window)
+        a.scale = dim ** -0.5 if self._scale is None else self._scale
         for name, t in zip(("q", "k", "v", "o", "d_o", "dq", "dk", "dv"), tensors):
             setattr(a, name, _token_strides(t))
+        _on_one_gpu(device, self.stream, *tensors, lse, *lengths)
         address = ctypes.addressof(a)
         count = (self._calls.h2x_attention_backward_workspace_bytes if gradients
                  else self._calls.h2x_attention_forward_workspace_bytes)
-        return self._plans.keep(key, (a, address, count(address)))
+        return self._plans.keep(key, (address, count(address), a))
 
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, output: torch.Tensor,
                 logsumexp: Optional[torch.Tensor] = None, query_lengths: Optional[torch.Tensor] = None,
                 key_lengths: Optional[torch.Tensor] = None) -> int:
         """logsumexp, (samples, heads, queries), is for the backward pass."""
-        _, address, nbytes = self._plan(query, key, value, output, logsumexp, (query_lengths, key_lengths))
-        _on_one_gpu(self.stream, query, key, value, output, logsumexp, query_lengths, key_lengths)
+        device = _current_device()
+        alike = _key(self._calls, device, query, key, value, output, logsumexp, query_lengths, key_lengths)
+        address, nbytes, _ = self._plans.get(alike) or self._plan(alike, device, query, key, value, output, logsumexp,
+                                                                  (query_lengths, key_lengths))
         ws = _buffer_of(self.stream, nbytes, torch.uint8) if nbytes else None
         status = self._calls.h2x_attention_forward(address, query, key, value, query_lengths, key_lengths, output, logsumexp, ws,
                                                    _stream_handle(self.stream))
@@ -322,11 +344,14 @@ class Attention:
                  d_value: torch.Tensor, query_lengths: Optional[torch.Tensor] = None,
                  key_lengths: Optional[torch.Tensor] = None) -> int:
         """Gradients, from the forward pass' output and logsumexp; they may not overlap the inputs."""
-        _require(logsumexp is not None, "the backward pass needs logsumexp")
-        _, address, nbytes = self._plan(query, key, value, output, logsumexp, (query_lengths, key_lengths),
-                                        (d_output, d_query, d_key, d_value))
-        _on_one_gpu(self.stream, query, key, value, output, d_output, logsumexp, d_query, d_key, d_value, query_lengths,
-                    key_lengths)
+        device = _current_device()
+        alike = _key(self._calls, device, query, key, value, output, d_output, logsumexp, d_query, d_key, d_value, query_lengths, key_lengths)
+        plan = self._plans.get(alike)
+        if plan is None:
+            _require(logsumexp is not None, "the backward pass needs logsumexp")
+            plan = self._plan(alike, device, query, key, value, output, logsumexp, (query_lengths, key_lengths),
+                              (d_output, d_query, d_key, d_value))
+        address, nbytes, _ = plan
         ws = _buffer_of(self.stream, nbytes, torch.uint8) if nbytes else None
         status = self._calls.h2x_attention_backward(address, query, key, value, output, d_output, logsumexp, query_lengths,
                                                     key_lengths, d_query, d_key, d_value, ws, _stream_handle(self.stream))
