@@ -271,33 +271,43 @@ __device__ __forceinline__ f32x16 zero16()
     return z;
 }
 
-// Element (m, n) = sum over DP of tile[first_row + m] * row n of the fragment: lane l's number i has n = l % 32 and
-// m = 8 (i / 4) + 4 (l / 32) + i % 4.
-template <typename T, int DP>
-__device__ __forceinline__ f32x16 product(LdsBytes tile, int first_row, const Fragment<T, DP>& f)
+// s[b] (m, n) = sum over DP of tile[first_row + 32 b + m] * row n of the fragment: lane l's number i has n = l % 32 and
+// m = 8 (i / 4) + 4 (l / 32) + i % 4.  (The blocks' chains of products are interleaved: none waits for its own last one.)
+template <typename T, int DP, int B>
+__device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fragment<T, DP>& f, f32x16 (&s)[B])
 {
     using L = Tile<T, DP>;
     const int lane = threadIdx.x & (kWaveSize - 1);
-    f32x16 s = zero16();
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+        s[b] = zero16();
 #pragma unroll
     for (int c = 0; c < L::kChunks / 2; ++c)
-    {
-        const LdsBytes at = tile + first_row * L::kRowBytes + L::address(lane & 31, 2 * c + lane / 32);
-        if constexpr (sizeof(T) == 2)
-        {
-            const bf16x8 a = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(at);
-            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, f.chunk[c]), s, 0, 0, 0);
-        }
-        else
-        {
-            const f32x4 a = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(at);
-            const f32x4 b = __builtin_bit_cast(f32x4, f.chunk[c]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                s = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], s, 0, 0, 0);
+        for (int b = 0; b < B; ++b)
+        {
+            const LdsBytes at = tile + (first_row + 32 * b) * L::kRowBytes + L::address(lane & 31, 2 * c + lane / 32);
+            if constexpr (sizeof(T) == 2)
+            {
+                const bf16x8 a = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(at);
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, f.chunk[c]), s[b], 0, 0, 0);
+            }
+            else
+            {
+                const f32x4 a = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(at);
+                const f32x4 w = __builtin_bit_cast(f32x4, f.chunk[c]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], w[i], s[b], 0, 0, 0);
+            }
         }
-    }
-    return s;
+}
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 product(LdsBytes tile, int first_row, const Fragment<T, DP>& f)
+{
+    f32x16 s[1];
+    products<T, DP>(tile, first_row, f, s);
+    return s[0];
 }
 
 // 32 x 32 numbers as they come out of product(), as second operand of a contraction over m.
@@ -403,6 +413,7 @@ __device__ __forceinline__ void store_row(T* p, int dim, const f32x16 (&v)[DP / 
 // [from, end).
 __device__ __forceinline__ void hide(f32x16* s, int first, int from, int end)
 {
+    asm volatile(""); // (most tiles are seen as a whole: a branch, no work that is thrown away)
     const int half = (threadIdx.x & (kWaveSize - 1)) / 32;
     const unsigned int seen = end > from ? end - from : 0;
     const int at = first + 4 * half - from;

@@ -58,9 +58,7 @@ struct Rows32
     // The scores of a tile's keys.
     __device__ __forceinline__ void score(LdsBytes k_tile, f32x16 (&s)[kTileKeys<T> / 32]) const
     {
-#pragma unroll
-        for (int b = 0; b < kTileKeys<T> / 32; ++b)
-            s[b] = product<T, DP>(k_tile, 32 * b, q);
+        products<T, DP>(k_tile, 0, q, s);
     }
 
     // Scores to probabilities, with maximum, sum and output brought up to date.
@@ -141,7 +139,7 @@ __device__ __forceinline__ void finish_row(const Args<T>& a, T* o, int64_t row, 
 // Many queries: the waves of a workgroup take 32 queries of a head each, and share the tiles of keys and values, which come
 // straight from memory to LDS while the tile before them is worked on.
 template <typename T, int DP, bool Whole>
-__global__ void __launch_bounds__(kThreads) attention_forward_kernel(const Args<T> a)
+__global__ void __launch_bounds__(kThreads, 2) attention_forward_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr int KT = kTileKeys<T>, kTileBytes = KT * Tile<T, DP>::kRowBytes;
