@@ -65,7 +65,44 @@ struct Sample
     }
 };
 
+// In which order workgroups go through the blocks of rows of all heads (of all samples).
+enum Order
+{
+    kByHead,     // head after head, each XCD a run of them: heads' keys and values stay in its L2
+    kFirstFirst, // the first blocks of all heads, which have the most to do, then the second ones ...
+    kLastFirst   // the same from the last ones on
+};
+struct Schedule
+{
+    Order order;
+    int fold; // blocks from this one on come the other way round
+};
+
 #ifdef __HIPCC__
+
+struct Place
+{
+    int head, block; // the head counted through all samples
+};
+// Of workgroup `id` of a grid of `grid`; heads from `heads` on have nothing to do.
+__device__ __forceinline__ Place place_of(const Schedule& s, uint32_t id, uint32_t grid, uint32_t heads, uint32_t blocks)
+{
+    if (s.order == kByHead)
+    {
+        id = xcd_contiguous(id, grid);
+        const uint32_t head = id / blocks;
+        return {static_cast<int>(head), static_cast<int>(id - head * blocks)};
+    }
+    uint32_t block = id / heads;
+    const uint32_t at = id - block * heads;
+    if (block >= blocks)
+        return {static_cast<int>(heads), 0};
+    if (block >= static_cast<uint32_t>(s.fold))
+        block = s.fold + blocks - 1 - block;
+    // workgroups of heads next to each other on one XCD, where the number of heads allows it
+    const uint32_t head = heads % kNumXcd == 0 ? at % kNumXcd * (heads / kNumXcd) + at / kNumXcd : at;
+    return {static_cast<int>(head), static_cast<int>(s.order == kFirstFirst ? block : blocks - 1 - block)};
+}
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -145,7 +182,19 @@ struct Tile
     {
         return row * kRowBytes + place(row, chunk) * 16;
     }
+    // Rows whose chunks are moved by exclusive or: so are addresses, by what chunk numbers differ in.
+    static constexpr bool kFlips = (kRowBytes & (kRowBytes - 1)) == 0;
 };
+
+// A number that the compiler does not know: what is worked out from it is worked out where it is used, and not kept in registers from
+// one round of a loop to the next.
+template <bool Lean>
+__device__ __forceinline__ int once(int v)
+{
+    if constexpr (Lean)
+        asm volatile("" : "+v"(v));
+    return v;
+}
 
 // A buffer of `rows` rows of `dim` elements, `stride` elements apart: reads behind it give zero.
 template <typename T>
@@ -273,11 +322,12 @@ __device__ __forceinline__ f32x16 zero16()
 
 // s[b] (m, n) = sum over DP of tile[first_row + 32 b + m] * row n of the fragment: lane l's number i has n = l % 32 and
 // m = 8 (i / 4) + 4 (l / 32) + i % 4.  (The blocks' chains of products are interleaved: none waits for its own last one.)
-template <typename T, int DP, int B>
+template <typename T, int DP, int B, bool Lean = false>
 __device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fragment<T, DP>& f, f32x16 (&s)[B])
 {
     using L = Tile<T, DP>;
     const int lane = threadIdx.x & (kWaveSize - 1);
+    const int base = once<Lean>(L::address(lane & 31, lane / 32));
 #pragma unroll
     for (int b = 0; b < B; ++b)
         s[b] = zero16();
@@ -286,7 +336,8 @@ __device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fra
 #pragma unroll
         for (int b = 0; b < B; ++b)
         {
-            const LdsBytes at = tile + (first_row + 32 * b) * L::kRowBytes + L::address(lane & 31, 2 * c + lane / 32);
+            const LdsBytes at = tile + (first_row + 32 * b) * L::kRowBytes
+                                + (L::kFlips ? base ^ 32 * c : L::address(lane & 31, 2 * c + lane / 32));
             if constexpr (sizeof(T) == 2)
             {
                 const bf16x8 a = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(at);
@@ -302,15 +353,51 @@ __device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fra
             }
         }
 }
-template <typename T, int DP>
+template <typename T, int DP, bool Lean = false>
 __device__ __forceinline__ f32x16 product(LdsBytes tile, int first_row, const Fragment<T, DP>& f)
 {
     f32x16 s[1];
-    products<T, DP>(tile, first_row, f, s);
+    products<T, DP, 1, Lean>(tile, first_row, f, s);
     return s[0];
 }
 
-// 32 x 32 numbers as they come out of product(), as second operand of a contraction over m.
+// The same of two tiles' rows with a fragment each, 32 rows: s from the first, t from the second.
+template <typename T, int DP, bool Lean = false>
+__device__ __forceinline__ void two_products(LdsBytes tile_s, LdsBytes tile_t, int first_row, const Fragment<T, DP>& f,
+                                             const Fragment<T, DP>& g, f32x16* s, f32x16* t)
+{
+    using L = Tile<T, DP>;
+    const int lane = threadIdx.x & (kWaveSize - 1);
+    const int base = once<Lean>(L::address(lane & 31, lane / 32));
+    *s = zero16();
+    *t = zero16();
+#pragma unroll
+    for (int c = 0; c < L::kChunks / 2; ++c)
+    {
+        const int at = first_row * L::kRowBytes + (L::kFlips ? base ^ 32 * c : L::address(lane & 31, 2 * c + lane / 32));
+        if constexpr (sizeof(T) == 2)
+        {
+            const bf16x8 a = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(tile_s + at);
+            const bf16x8 b = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(tile_t + at);
+            *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, f.chunk[c]), *s, 0, 0, 0);
+            *t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b, __builtin_bit_cast(bf16x8, g.chunk[c]), *t, 0, 0, 0);
+        }
+        else
+        {
+            const f32x4 a = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(tile_s + at);
+            const f32x4 b = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(tile_t + at);
+            const f32x4 u = __builtin_bit_cast(f32x4, f.chunk[c]), v = __builtin_bit_cast(f32x4, g.chunk[c]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                *s = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], u[i], *s, 0, 0, 0);
+                *t = __builtin_amdgcn_mfma_f32_32x32x2f32(b[i], v[i], *t, 0, 0, 0);
+            }
+        }
+    }
+}
+
+// 32 x 32 numbers as they come out of products(), as second operand of a contraction over m.
 template <typename T>
 struct Weights;
 template <>
@@ -327,7 +414,7 @@ struct Weights<float>
 };
 
 // out[d] (e, n) += sum over m of tile[first_row + m][32 d + e] * w(m, n), for the DP / 32 blocks of elements.
-template <int DP>
+template <int DP, bool Lean = false>
 __device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const Weights<bf16>& w, f32x16 (&out)[DP / 32])
 {
     using L = Tile<bf16, DP>;
@@ -336,6 +423,7 @@ __device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const W
     // transposing load gives 16 lanes 16 columns of four rows, lane j having loaded four columns of row j / 4.
     const int row = 4 * (lane / 32) + (lane & 15) / 4;
     const int chunk = (lane & 16) / 8 + (lane & 3) / 2, byte = (lane & 1) * 8;
+    const int base = once<Lean>(L::address(row, chunk) + byte);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -347,7 +435,8 @@ __device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const W
             {
                 const LdsBytes at =
                     tile + (first_row + 16 * t + 8 * u) * L::kRowBytes
-                    + (row * L::kRowBytes + L::place(16 * t + 8 * u + row, 4 * d + chunk) * 16 + byte);
+                    + (L::kFlips ? base ^ (64 * d + 32 * u) // (rows 8 further on are moved by two chunks more)
+                                 : row * L::kRowBytes + L::place(16 * t + 8 * u + row, 4 * d + chunk) * 16 + byte);
                 const bf16x4 part = __builtin_bit_cast(
                     bf16x4,
                     __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(at)));
@@ -358,7 +447,7 @@ __device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const W
             out[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w.v[t], out[d], 0, 0, 0);
         }
 }
-template <int DP>
+template <int DP, bool Lean = false>
 __device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const Weights<float>& w, f32x16 (&out)[DP / 32])
 {
     using L = Tile<float, DP>;
@@ -477,6 +566,17 @@ inline Masks masks_of(const h2x_attention& a, const int32_t* query_lengths, cons
             static_cast<int32_t>(a.keys),
             bound(a.window_left),
             bound(a.window_right)};
+}
+
+// The order for blocks of queries, or of keys, which are the other way round.  Under a mask that bounds one side blocks have unlike numbers of
+// tiles: the longest first, so that the short ones fill up the end.  Where all workgroups run at once, two a CU, the second one of a CU is the
+// shorter the longer its first.
+inline Schedule schedule_of(const h2x_attention& a, bool keys, uint64_t heads, uint64_t blocks)
+{
+    const bool left = a.window_left >= 0, right = a.window_right >= 0;
+    if (left == right)
+        return {kByHead, 0};
+    return {right != keys ? kLastFirst : kFirstFirst, static_cast<int>(blocks)};
 }
 
 // f(std::integral_constant<int, DP>) for heads padded to a multiple of 32 elements.

@@ -16,6 +16,10 @@ namespace
 template <typename T>
 constexpr int kTileRows = sizeof(T) == 2 ? 64 : 32;
 
+// Waves that a SIMD is to have: two, so that one's exponentials run beside the other's products, where 256 registers hold the rows.
+template <typename T, int DP, bool Whole>
+constexpr int kWavesOf = Whole && (sizeof(T) == 2 || DP <= 64) ? 2 : 1;
+
 template <typename T>
 struct Args
 {
@@ -27,8 +31,9 @@ struct Args
     Strides qs, ks, vs, os, d_os, dqs, dks, dvs;
     Masks masks;
     float scale, scale_log2;
-    int dim, query_heads, group, blocks;
-    uint32_t total; // workgroups that have work
+    int dim, query_heads, group;
+    int blocks, heads; // of rows in a head, and heads in all samples
+    Schedule schedule;
 };
 
 // Sum of products of two fragments' elements, over both halves.
@@ -49,16 +54,15 @@ __device__ __forceinline__ float dot(const Fragment<T, DP>& a, const Fragment<T,
 
 // dq, and what the other pass needs of each row.  As in the forward pass, the waves of a workgroup take 32 queries of a head each.
 template <typename T, int DP, bool Whole>
-__global__ void __launch_bounds__(kThreads) attention_dq_kernel(const Args<T> a)
+__global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_dq_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr int KT = kTileRows<T>, kTileBytes = KT * Tile<T, DP>::kRowBytes;
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
-    const uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
-    if (id >= a.total)
+    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks);
+    if (place.head >= a.heads)
         return;
-    const int block = a.blocks - 1 - id % a.blocks; // (the longest first under a causal mask)
-    const int head = id / a.blocks % a.query_heads, n = id / a.blocks / a.query_heads;
+    const int block = place.block, n = place.head / a.query_heads, head = place.head - n * a.query_heads;
     const int lane = threadIdx.x & (kWaveSize - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const Sample sample = sample_of(a.masks, n);
 
@@ -127,8 +131,8 @@ __global__ void __launch_bounds__(kThreads) attention_dq_kernel(const Args<T> a)
             const int at = from + tile * KT + 32 * b;
             if (first > last || at >= some_end || at + 32 <= some_from)
                 continue;
-            f32x16 s = product<T, DP>(k_tile, 32 * b, q);
-            const f32x16 dp = product<T, DP>(v_tile, 32 * b, d_o);
+            f32x16 s, dp;
+            two_products<T, DP>(k_tile, v_tile, 32 * b, q, d_o, &s, &dp);
             if (at < all_from || at + 32 > all_end)
                 hide(&s, at, row_from, row_end);
             Weights<T> ds;
@@ -149,18 +153,18 @@ __global__ void __launch_bounds__(kThreads) attention_dq_kernel(const Args<T> a)
 // dk and dv: the waves of a workgroup take 32 keys of a key head each; the queries of the heads that share it pass through LDS, one head after
 // another.
 template <typename T, int DP, bool Whole>
-__global__ void __launch_bounds__(kThreads) attention_dkv_kernel(const Args<T> a)
+__global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Whole>)) attention_dkv_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
+    constexpr bool kLean = false; // its rows leave no registers for addresses
     constexpr int QT = kTileRows<T>, kTileBytes = QT * Tile<T, DP>::kRowBytes;
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kWaveSize];
-    const uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
-    if (id >= a.total)
-        return;
     const int key_heads = a.query_heads / a.group;
-    const int block = id % a.blocks; // (under a causal mask the first keys have the most queries)
-    const int key_head = id / a.blocks % key_heads, n = id / a.blocks / key_heads;
+    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks);
+    if (place.head >= a.heads)
+        return;
+    const int block = place.block, n = place.head / key_heads, key_head = place.head - n * key_heads;
     const int lane = threadIdx.x & (kWaveSize - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const Sample sample = sample_of(a.masks, n);
 
@@ -224,14 +228,16 @@ __global__ void __launch_bounds__(kThreads) attention_dkv_kernel(const Args<T> a
             const int at = here + 32 * b;
             if (first > last || at >= some_end || at + 32 <= some_from)
                 continue;
-            f32x16 s = product<T, DP>(q_tile, 32 * b, k);
+            const float* const log2_sum = &stats[stage][0][32 * b + 4 * (lane / 32)];
+            const float* const delta = &stats[stage][1][32 * b + 4 * (lane / 32)];
+            Weights<T> p, ds;
+            f32x16 s = product<T, DP, kLean>(q_tile, 32 * b, k);
             if (at < all_from || at + 32 > all_end)
                 hide(&s, at, row_from, row_end);
-            Weights<T> p, ds;
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
             {
-                const f32x4 l = *reinterpret_cast<const f32x4*>(&stats[stage][0][32 * b + 2 * r + 4 * (lane / 32)]);
+                const f32x4 l = *reinterpret_cast<const f32x4*>(log2_sum + 2 * r);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                 {
@@ -239,17 +245,17 @@ __global__ void __launch_bounds__(kThreads) attention_dkv_kernel(const Args<T> a
                     p.set(r + e, s[r + e]);
                 }
             }
-            accumulate<DP>(d_o_tile, 32 * b, p, dv);
-            const f32x16 dp = product<T, DP>(d_o_tile, 32 * b, v);
+            accumulate<DP, kLean>(d_o_tile, 32 * b, p, dv);
+            const f32x16 dp = product<T, DP, kLean>(d_o_tile, 32 * b, v);
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
             {
-                const f32x4 delta = *reinterpret_cast<const f32x4*>(&stats[stage][1][32 * b + 2 * r + 4 * (lane / 32)]);
+                const f32x4 l = *reinterpret_cast<const f32x4*>(delta + 2 * r);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    ds.set(r + e, s[r + e] * (dp[r + e] - delta[e]));
+                    ds.set(r + e, s[r + e] * (dp[r + e] - l[e]));
             }
-            accumulate<DP>(q_tile, 32 * b, ds, dk);
+            accumulate<DP, kLean>(q_tile, 32 * b, ds, dk);
         }
     }
     if (j < a.masks.keys)
@@ -287,13 +293,15 @@ int issue(const h2x_attention& c, Args<T> a, hipStream_t stream)
         if (query_groups > 0)
         {
             a.blocks = static_cast<int>(query_blocks);
-            a.total = static_cast<uint32_t>(query_groups);
+            a.heads = c.samples * c.query_heads;
+            a.schedule = schedule_of(c, false, a.heads, query_blocks);
             launch(attention_dq_kernel<T, DP, Whole>, grid(query_groups), dim3(kThreads), stream, a);
         }
         if (key_groups > 0)
         {
             a.blocks = static_cast<int>(key_blocks);
-            a.total = static_cast<uint32_t>(key_groups);
+            a.heads = c.samples * c.key_heads;
+            a.schedule = schedule_of(c, true, a.heads, key_blocks);
             launch(attention_dkv_kernel<T, DP, Whole>, grid(key_groups), dim3(kThreads), stream, a);
         }
         return launch_status();

@@ -34,7 +34,8 @@ struct Args
     Parts parts;
     float scale_log2;
     int dim, samples, query_heads, group, query_blocks;
-    uint32_t total; // workgroups that have work
+    int heads; // of all samples; few queries: key heads
+    Schedule schedule;
 };
 
 // A wave's 32 rows.
@@ -144,14 +145,11 @@ __global__ void __launch_bounds__(kThreads, 2) attention_forward_kernel(const Ar
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr int KT = kTileKeys<T>, kTileBytes = KT * Tile<T, DP>::kRowBytes;
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
-    const uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
-    if (id >= a.total)
+    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.query_blocks * a.parts.num);
+    if (place.head >= a.heads)
         return;
-    const int part = id % a.parts.num;
-    const uint32_t of_head = id / a.parts.num;
-    // the last queries first: under a causal mask they have the most keys
-    const int block = a.query_blocks - 1 - of_head % a.query_blocks;
-    const int head = of_head / a.query_blocks % a.query_heads, n = of_head / a.query_blocks / a.query_heads;
+    const int block = place.block / a.parts.num, part = place.block - block * a.parts.num;
+    const int n = place.head / a.query_heads, head = place.head - n * a.query_heads;
     const int lane = threadIdx.x & (kWaveSize - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const Sample sample = sample_of(a.masks, n);
 
@@ -230,14 +228,12 @@ __global__ void __launch_bounds__(kThreads) attention_few_kernel(const Args<T> a
     constexpr int kJoinBytes = kWaves * kRows * kJoinStride * 4, kTilesBytes = kWaves * 2 * kTileBytes;
     __shared__ __attribute__((aligned(16))) char lds[kTilesBytes > kJoinBytes ? kTilesBytes : kJoinBytes];
     __shared__ float max_sum[kWaves][kRows][2];
-    const uint32_t id = xcd_contiguous(blockIdx.x, gridDim.x);
-    if (id >= a.total)
+    const Place place = place_of({kByHead, 0}, blockIdx.x, gridDim.x, a.heads, a.query_blocks * a.parts.num);
+    if (place.head >= a.heads)
         return;
-    const int part = id % a.parts.num;
-    const uint32_t of_head = id / a.parts.num;
     const int key_heads = a.query_heads / a.group;
-    const int block = of_head % a.query_blocks, key_head = of_head / a.query_blocks % key_heads;
-    const int n = of_head / a.query_blocks / key_heads;
+    const int block = place.block / a.parts.num, part = place.block - block * a.parts.num;
+    const int n = place.head / key_heads, key_head = place.head - n * key_heads;
     const int lane = threadIdx.x & (kWaveSize - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const Sample sample = sample_of(a.masks, n);
 
@@ -543,7 +539,8 @@ extern "C" int h2x_attention_forward(const h2x_attention* attention, const void*
         a.query_heads = c.query_heads;
         a.group = c.query_heads / c.key_heads;
         a.query_blocks = p.query_blocks;
-        a.total = static_cast<uint32_t>(p.groups);
+        a.heads = c.samples * (p.few ? c.key_heads : c.query_heads);
+        a.schedule = schedule_of(c, false, a.heads, static_cast<uint64_t>(p.query_blocks) * p.parts);
         return issue<T, decltype(is_whole)::value>(c, p, a, as_stream(stream));
     });
 }
