@@ -5,8 +5,13 @@
 // contracted dimension.  Tiles of the other side pass through LDS, shared by the workgroup.  With the other side as the
 // first operand, a tile of scores comes out with a lane's 16 numbers in its own row: sums and maxima along a row are made in
 // the lane (and once across the halves), and the probabilities are the second operand of the next product as they lie.
-// That product contracts over the other side's rows, so its first operand is the same tile in LDS read across:
-// 16-bit elements by the transposing LDS loads, 32-bit ones singly.
+// That product contracts over the other side's rows, so its first operand is the same tile in LDS read across, by the
+// transposing LDS loads.
+//
+// Products are of 16-bit numbers, summed in 32 bits.  A float is three of them, each the rounding of what those before it leave: eight bits each,
+// all 24.  Of the nine products of two floats the six that reach 2^-18 of the largest are made; the other three are together below
+// 2^-24, half a step of a float.  Six products of 16-bit numbers take three eighths of the time of one by the matrix units' 32-bit
+// form.
 #pragma once
 
 #include "h2x_token.hpp"
@@ -132,14 +137,93 @@ __device__ __forceinline__ float halves_sum(float v)
     return combine_apart<32>(v, [](float a, float b) { return a + b; });
 }
 
+// ---- elements ------------------------------------------------------------------------------------------------
+template <typename T>
+constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3; // 16-bit numbers of an element
+
+// x as a sum of 16-bit numbers, largest first.
+__device__ __forceinline__ void split(float x, bf16 (&v)[3])
+{
+    v[0] = static_cast<bf16>(x);
+    x -= static_cast<float>(v[0]);
+    v[1] = static_cast<bf16>(x);
+    x -= static_cast<float>(v[1]);
+    v[2] = static_cast<bf16>(x);
+}
+
+// Eight neighbouring elements as they come from memory.
+template <typename T>
+struct Eight;
+template <>
+struct Eight<bf16>
+{
+    u32x4 v;
+};
+template <>
+struct Eight<float>
+{
+    u32x4 v[2];
+};
+__device__ __forceinline__ void planes_of(const Eight<bf16>& e, bf16x8 (&out)[1])
+{
+    out[0] = __builtin_bit_cast(bf16x8, e.v);
+}
+__device__ __forceinline__ void planes_of(const Eight<float>& e, bf16x8 (&out)[3])
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        bf16 parts[3];
+        split(__uint_as_float(e.v[i / 4][i % 4]), parts);
+        out[0][i] = parts[0];
+        out[1][i] = parts[1];
+        out[2][i] = parts[2];
+    }
+}
+__device__ __forceinline__ float element(const Eight<bf16>& e, int i)
+{
+    return static_cast<float>(__builtin_bit_cast(bf16x8, e.v)[i]);
+}
+__device__ __forceinline__ float element(const Eight<float>& e, int i)
+{
+    return __uint_as_float(e.v[i / 4][i % 4]);
+}
+
+// Elements at .. at + 7 of the row at p; zero from dim on, and where the row is not `there`.
+template <typename T, bool Whole>
+__device__ __forceinline__ Eight<T> load_eight(const T* p, int at, bool there, int dim)
+{
+    constexpr int N = 16 / sizeof(T);
+    u32x4 v[8 / N];
+#pragma unroll
+    for (int n = 0; n < 8 / N; ++n, at += N)
+    {
+        v[n] = u32x4{0, 0, 0, 0};
+        if constexpr (Whole)
+        {
+            if (there && at < dim)
+                v[n] = *reinterpret_cast<const u32x4*>(p + at);
+        }
+        else
+        {
+            AVec<T, N> x;
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                x.v[i] = there && at + i < dim ? p[at + i] : static_cast<T>(0.0f);
+            v[n] = __builtin_bit_cast(u32x4, x);
+        }
+    }
+    return __builtin_bit_cast(Eight<T>, v);
+}
+
 // ---- tiles in LDS ------------------------------------------------------------------------------------------
-// A tile of rows of DP elements, in 16-byte chunks.  Chunks are moved about within their row so that both ways of reading
-// find their lanes' data on different banks: 16 rows at the same chunk (16 bytes a lane), and 4 rows (row % 4 = 0 .. 3) at
-// 4 neighbouring chunks (8 bytes a lane).
-template <typename T, int DP>
+// A tile of R rows of DP 16-bit numbers, in 16-byte chunks; of floats three such, one behind the other.  Chunks are moved about within their row
+// so that both ways of reading find their lanes' data on different banks: 16 rows at the same chunk (16 bytes a lane), and 4 rows (row % 4 =
+// 0 .. 3) at 4 neighbouring chunks (8 bytes a lane).
+template <int DP>
 struct Tile
 {
-    static constexpr int kRowBytes = DP * sizeof(T), kChunks = kRowBytes / 16, kPerChunk = 16 / sizeof(T);
+    static constexpr int kRowBytes = DP * 2, kChunks = DP / 8;
 
     __device__ static __forceinline__ int place(int row, int chunk)
     {
@@ -152,15 +236,8 @@ struct Tile
             const int at = chunk + ((row >> 2) & 3);
             return at >= kChunks ? at - kChunks : at;
         }
-        else if constexpr (kRowBytes == 256)
-            return chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
-        else if constexpr (kRowBytes == 384)
-        {
-            const int at = chunk + ((row >> 1) & 7);
-            return at >= kChunks ? at - kChunks : at;
-        }
         else
-            return chunk ^ (row & 15);
+            return chunk ^ (((row & 3) << 2) | ((row >> 2) & 3));
     }
     // The chunk that lies at a place.
     __device__ static __forceinline__ int chunk_at(int row, int at)
@@ -168,11 +245,6 @@ struct Tile
         if constexpr (kRowBytes == 192)
         {
             const int chunk = at - ((row >> 2) & 3);
-            return chunk < 0 ? chunk + kChunks : chunk;
-        }
-        else if constexpr (kRowBytes == 384)
-        {
-            const int chunk = at - ((row >> 1) & 7);
             return chunk < 0 ? chunk + kChunks : chunk;
         }
         else
@@ -185,16 +257,8 @@ struct Tile
     // Rows whose chunks are moved by exclusive or: so are addresses, by what chunk numbers differ in.
     static constexpr bool kFlips = (kRowBytes & (kRowBytes - 1)) == 0;
 };
-
-// A number that the compiler does not know: what is worked out from it is worked out where it is used, and not kept in registers from
-// one round of a loop to the next.
-template <bool Lean>
-__device__ __forceinline__ int once(int v)
-{
-    if constexpr (Lean)
-        asm volatile("" : "+v"(v));
-    return v;
-}
+template <typename T, int DP, int R>
+constexpr int kTileBytes = kPlanes<T>* R* Tile<DP>::kRowBytes;
 
 // A buffer of `rows` rows of `dim` elements, `stride` elements apart: reads behind it give zero.
 template <typename T>
@@ -204,64 +268,6 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const T* p, int rows
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, static_cast<int>(bytes), 0x00020000);
 }
 constexpr unsigned int kOutside = 0x80000000u; // behind every buffer
-
-// One 16-byte chunk of a row that may begin on any element.
-template <typename T>
-__device__ __forceinline__ u32x4 load_elements(__amdgpu_buffer_rsrc_t b, int row, int chunk, int stride_bytes, int dim)
-{
-    constexpr int N = 16 / sizeof(T);
-    const unsigned int at = row * stride_bytes + chunk * 16;
-    u32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-    {
-        if constexpr (sizeof(T) == 4)
-            v[i] = __builtin_amdgcn_raw_buffer_load_b32(b, chunk * N + i < dim ? at + 4 * i : kOutside, 0, 0);
-        else
-        {
-            const unsigned int lo = static_cast<unsigned short>(
-                __builtin_amdgcn_raw_buffer_load_b16(b, chunk * N + 2 * i < dim ? at + 4 * i : kOutside, 0, 0));
-            const unsigned int hi = static_cast<unsigned short>(
-                __builtin_amdgcn_raw_buffer_load_b16(b, chunk * N + 2 * i + 1 < dim ? at + 4 * i + 2 : kOutside, 0, 0));
-            v[i] = lo | hi << 16;
-        }
-    }
-    return v;
-}
-
-// Loads R rows of a buffer into a tile, by Threads threads (t: this one's number among them).  Whole chunks go straight to LDS, and
-// are there when the wave that loads them has waited for its loads; others through registers, and are there after a barrier.
-template <typename T, int DP, int R, int Threads, bool Whole>
-__device__ __forceinline__ void load_tile(__amdgpu_buffer_rsrc_t b, int stride_bytes, int dim, LdsBytes tile, int t)
-{
-    using L = Tile<T, DP>;
-    constexpr int kTotal = R * L::kChunks;
-    static_assert(kTotal % kWaveSize == 0, "whole waves");
-#pragma unroll
-    for (int i = 0; i < kTotal; i += Threads)
-    {
-        const int p = i + t;
-        if (kTotal % Threads != 0 && i + (t & ~(kWaveSize - 1)) >= kTotal)
-            break;
-        const int row = p / L::kChunks, chunk = L::chunk_at(row, p % L::kChunks);
-        if constexpr (Whole)
-        {
-            const unsigned int at = row * stride_bytes + chunk * 16;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                b, reinterpret_cast<__attribute__((address_space(3))) void*>(tile + (i + (t & ~(kWaveSize - 1))) * 16), 16,
-                chunk * L::kPerChunk < dim ? at : kOutside, 0, 0, 0);
-        }
-        else
-            *reinterpret_cast<__attribute__((address_space(3))) u32x4*>(tile + p * 16) =
-                load_elements<T>(b, row, chunk, stride_bytes, dim);
-    }
-}
-
-// 64 numbers of a buffer to LDS, by a wave.
-__device__ __forceinline__ void load_numbers(__amdgpu_buffer_rsrc_t b, LdsBytes to, int lane)
-{
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, reinterpret_cast<__attribute__((address_space(3))) void*>(to), 4, lane * 4, 0, 0, 0);
-}
 
 // Until no more than N of this wave's loads are under way (they arrive in order).
 template <int N = 0>
@@ -275,40 +281,98 @@ __device__ __forceinline__ void wait_for_lds()
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
 }
 
+// How Threads threads (t: this one's number among them) bring R rows of a buffer into a tile.  Whole chunks of 16-bit elements go
+// straight to LDS, and are there when the wave that has issued the loads has waited for them; others are held in registers until they are put there.
+template <typename T, int DP, int R, int Threads, bool Whole>
+struct TileLoad
+{
+    static constexpr bool kDirect = Whole && sizeof(T) == 2;
+    static constexpr int kUnits = R * Tile<DP>::kChunks, kEach = (kUnits + Threads - 1) / Threads; // of eight elements
+    static_assert(kUnits % kWaveSize == 0, "whole waves");
+    Eight<T> held[kDirect ? 1 : kEach];
+
+    __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t b, int stride_bytes, int dim, LdsBytes tile, int t)
+    {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+        {
+            const int p = i * Threads + t, of_wave = i * Threads + (t & ~(kWaveSize - 1));
+            if (kUnits % Threads != 0 && of_wave >= kUnits)
+                break;
+            const int row = p / Tile<DP>::kChunks, at = 8 * Tile<DP>::chunk_at(row, p % Tile<DP>::kChunks);
+            const unsigned int byte = row * stride_bytes + at * static_cast<int>(sizeof(T));
+            if constexpr (kDirect)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    b, reinterpret_cast<__attribute__((address_space(3))) void*>(tile + of_wave * 16), 16, at < dim ? byte : kOutside, 0,
+                    0, 0);
+            else if constexpr (Whole)
+            {
+                held[i].v[0] = __builtin_amdgcn_raw_buffer_load_b128(b, at < dim ? byte : kOutside, 0, 0);
+                held[i].v[1] = __builtin_amdgcn_raw_buffer_load_b128(b, at + 4 < dim ? byte + 16 : kOutside, 0, 0);
+            }
+            else if constexpr (sizeof(T) == 4)
+            {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    held[i].v[j / 4][j % 4] = __builtin_amdgcn_raw_buffer_load_b32(b, at + j < dim ? byte + 4 * j : kOutside, 0, 0);
+            }
+            else
+            {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    const unsigned int lo = static_cast<unsigned short>(
+                        __builtin_amdgcn_raw_buffer_load_b16(b, at + 2 * j < dim ? byte + 4 * j : kOutside, 0, 0));
+                    const unsigned int hi = static_cast<unsigned short>(
+                        __builtin_amdgcn_raw_buffer_load_b16(b, at + 2 * j + 1 < dim ? byte + 4 * j + 2 : kOutside, 0, 0));
+                    held[i].v[j] = lo | hi << 16;
+                }
+            }
+        }
+    }
+
+    // (The tile is there for other waves after a barrier.)
+    __device__ __forceinline__ void put(LdsBytes tile, int t) const
+    {
+        if constexpr (!kDirect)
+        {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i)
+            {
+                if (kUnits % Threads != 0 && i * Threads + (t & ~(kWaveSize - 1)) >= kUnits)
+                    break;
+                bf16x8 planes[kPlanes<T>];
+                planes_of(held[i], planes);
+#pragma unroll
+                for (int p = 0; p < kPlanes<T>; ++p)
+                    *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(tile + (p * kUnits + i * Threads + t) * 16) = planes[p];
+            }
+        }
+    }
+};
+
+// 64 numbers of a buffer to LDS, by a wave.
+__device__ __forceinline__ void load_numbers(__amdgpu_buffer_rsrc_t b, LdsBytes to, int lane)
+{
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, reinterpret_cast<__attribute__((address_space(3))) void*>(to), 4, lane * 4, 0, 0, 0);
+}
+
 // ---- products --------------------------------------------------------------------------------------------------
 // A row's elements as second operand: what lane l has of row l % 32, for the contraction over DP elements.
 template <typename T, int DP>
 struct Fragment
 {
-    u32x4 chunk[Tile<T, DP>::kChunks / 2]; // chunks 2 c + (lane / 32)
+    bf16x8 chunk[DP / 16][kPlanes<T>]; // elements 16 c + 8 (lane / 32) and on
 };
 
 // Of the row at p; zero where it is not `there`.
 template <typename T, int DP, bool Whole>
 __device__ __forceinline__ void load_fragment(Fragment<T, DP>* f, const T* p, bool there, int dim)
 {
-    constexpr int N = 16 / sizeof(T);
     const int half = (threadIdx.x & (kWaveSize - 1)) / 32;
 #pragma unroll
-    for (int c = 0; c < Tile<T, DP>::kChunks / 2; ++c)
-    {
-        const int at = (2 * c + half) * N;
-        u32x4 v = {0, 0, 0, 0};
-        if constexpr (Whole)
-        {
-            if (there && at < dim)
-                v = *reinterpret_cast<const u32x4*>(p + at);
-        }
-        else
-        {
-            AVec<T, N> x;
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                x.v[i] = there && at + i < dim ? p[at + i] : static_cast<T>(0.0f);
-            v = __builtin_bit_cast(u32x4, x);
-        }
-        f->chunk[c] = v;
-    }
+    for (int c = 0; c < DP / 16; ++c)
+        planes_of(load_eight<T, Whole>(p, 16 * c + 8 * half, there, dim), f->chunk[c]);
 }
 
 __device__ __forceinline__ f32x16 zero16()
@@ -320,150 +384,134 @@ __device__ __forceinline__ f32x16 zero16()
     return z;
 }
 
-// s[b] (m, n) = sum over DP of tile[first_row + 32 b + m] * row n of the fragment: lane l's number i has n = l % 32 and
+__device__ __forceinline__ void multiply(const bf16x8 (&a)[1], const bf16x8 (&b)[1], f32x16* s)
+{
+    *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], *s, 0, 0, 0);
+}
+__device__ __forceinline__ void multiply(const bf16x8 (&a)[3], const bf16x8 (&b)[3], f32x16* s)
+{
+    *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[2], b[0], *s, 0, 0, 0); // (small ones first)
+    *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[2], *s, 0, 0, 0);
+    *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[1], *s, 0, 0, 0);
+    *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[1], b[0], *s, 0, 0, 0);
+    *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[1], *s, 0, 0, 0);
+    *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], *s, 0, 0, 0);
+}
+
+// s[b] (m, n) = sum over DP of tile[first_row + 32 b + m] * row n of the fragment, of a tile of R rows: lane l's number i has n = l % 32 and
 // m = 8 (i / 4) + 4 (l / 32) + i % 4.  (The blocks' chains of products are interleaved: none waits for its own last one.)
-template <typename T, int DP, int B, bool Lean = false>
+template <typename T, int DP, int R, int B>
 __device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fragment<T, DP>& f, f32x16 (&s)[B])
 {
-    using L = Tile<T, DP>;
+    using L = Tile<DP>;
     const int lane = threadIdx.x & (kWaveSize - 1);
-    const int base = once<Lean>(L::address(lane & 31, lane / 32));
+    const int base = L::address(lane & 31, lane / 32);
 #pragma unroll
     for (int b = 0; b < B; ++b)
         s[b] = zero16();
 #pragma unroll
-    for (int c = 0; c < L::kChunks / 2; ++c)
+    for (int c = 0; c < DP / 16; ++c)
 #pragma unroll
         for (int b = 0; b < B; ++b)
         {
             const LdsBytes at = tile + (first_row + 32 * b) * L::kRowBytes
                                 + (L::kFlips ? base ^ 32 * c : L::address(lane & 31, 2 * c + lane / 32));
-            if constexpr (sizeof(T) == 2)
-            {
-                const bf16x8 a = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(at);
-                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, f.chunk[c]), s[b], 0, 0, 0);
-            }
-            else
-            {
-                const f32x4 a = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(at);
-                const f32x4 w = __builtin_bit_cast(f32x4, f.chunk[c]);
+            bf16x8 a[kPlanes<T>];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], w[i], s[b], 0, 0, 0);
-            }
+            for (int p = 0; p < kPlanes<T>; ++p)
+                a[p] = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(at + p * R * L::kRowBytes);
+            multiply(a, f.chunk[c], &s[b]);
         }
 }
-template <typename T, int DP, bool Lean = false>
+template <typename T, int DP, int R>
 __device__ __forceinline__ f32x16 product(LdsBytes tile, int first_row, const Fragment<T, DP>& f)
 {
     f32x16 s[1];
-    products<T, DP, 1, Lean>(tile, first_row, f, s);
+    products<T, DP, R>(tile, first_row, f, s);
     return s[0];
 }
 
 // The same of two tiles' rows with a fragment each, 32 rows: s from the first, t from the second.
-template <typename T, int DP, bool Lean = false>
+template <typename T, int DP, int R>
 __device__ __forceinline__ void two_products(LdsBytes tile_s, LdsBytes tile_t, int first_row, const Fragment<T, DP>& f,
                                              const Fragment<T, DP>& g, f32x16* s, f32x16* t)
 {
-    using L = Tile<T, DP>;
+    using L = Tile<DP>;
     const int lane = threadIdx.x & (kWaveSize - 1);
-    const int base = once<Lean>(L::address(lane & 31, lane / 32));
+    const int base = L::address(lane & 31, lane / 32);
     *s = zero16();
     *t = zero16();
 #pragma unroll
-    for (int c = 0; c < L::kChunks / 2; ++c)
+    for (int c = 0; c < DP / 16; ++c)
     {
         const int at = first_row * L::kRowBytes + (L::kFlips ? base ^ 32 * c : L::address(lane & 31, 2 * c + lane / 32));
-        if constexpr (sizeof(T) == 2)
-        {
-            const bf16x8 a = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(tile_s + at);
-            const bf16x8 b = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(tile_t + at);
-            *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, __builtin_bit_cast(bf16x8, f.chunk[c]), *s, 0, 0, 0);
-            *t = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b, __builtin_bit_cast(bf16x8, g.chunk[c]), *t, 0, 0, 0);
-        }
-        else
-        {
-            const f32x4 a = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(tile_s + at);
-            const f32x4 b = *reinterpret_cast<__attribute__((address_space(3))) f32x4*>(tile_t + at);
-            const f32x4 u = __builtin_bit_cast(f32x4, f.chunk[c]), v = __builtin_bit_cast(f32x4, g.chunk[c]);
+        bf16x8 a[kPlanes<T>], b[kPlanes<T>];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-            {
-                *s = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], u[i], *s, 0, 0, 0);
-                *t = __builtin_amdgcn_mfma_f32_32x32x2f32(b[i], v[i], *t, 0, 0, 0);
-            }
+        for (int p = 0; p < kPlanes<T>; ++p)
+        {
+            a[p] = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(tile_s + at + p * R * L::kRowBytes);
+            b[p] = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(tile_t + at + p * R * L::kRowBytes);
         }
+        multiply(a, f.chunk[c], s);
+        multiply(b, g.chunk[c], t);
     }
 }
 
 // 32 x 32 numbers as they come out of products(), as second operand of a contraction over m.
 template <typename T>
-struct Weights;
-template <>
-struct Weights<bf16>
+struct Weights
 {
-    bf16x8 v[2];
-    __device__ __forceinline__ void set(int i, float x) { v[i / 8][i % 8] = static_cast<bf16>(x); }
-};
-template <>
-struct Weights<float>
-{
-    float v[16];
-    __device__ __forceinline__ void set(int i, float x) { v[i] = x; }
+    bf16x8 v[2][kPlanes<T>];
+    __device__ __forceinline__ void set(int i, float x)
+    {
+        if constexpr (kPlanes<T> == 1)
+            v[i / 8][0][i % 8] = static_cast<bf16>(x);
+        else
+        {
+            bf16 parts[3];
+            split(x, parts);
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+                v[i / 8][p][i % 8] = parts[p];
+        }
+    }
 };
 
 // out[d] (e, n) += sum over m of tile[first_row + m][32 d + e] * w(m, n), for the DP / 32 blocks of elements.
-template <int DP, bool Lean = false>
-__device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const Weights<bf16>& w, f32x16 (&out)[DP / 32])
+template <typename T, int DP, int R>
+__device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const Weights<T>& w, f32x16 (&out)[DP / 32])
 {
-    using L = Tile<bf16, DP>;
+    using L = Tile<DP>;
     const int lane = threadIdx.x & (kWaveSize - 1);
     // Number i of half h is row 8 (i / 4) + 4 h + i % 4: eight of them, as one operand holds, are two runs of four rows.  A
     // transposing load gives 16 lanes 16 columns of four rows, lane j having loaded four columns of row j / 4.
     const int row = 4 * (lane / 32) + (lane & 15) / 4;
     const int chunk = (lane & 16) / 8 + (lane & 3) / 2, byte = (lane & 1) * 8;
-    const int base = once<Lean>(L::address(row, chunk) + byte);
+    const int base = L::address(row, chunk) + byte;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int t = 0; t < 2; ++t)
         {
-            bf16x8 a;
+            bf16x8 a[kPlanes<T>];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-            {
-                const LdsBytes at =
-                    tile + (first_row + 16 * t + 8 * u) * L::kRowBytes
-                    + (L::kFlips ? base ^ (64 * d + 32 * u) // (rows 8 further on are moved by two chunks more)
-                                 : row * L::kRowBytes + L::place(16 * t + 8 * u + row, 4 * d + chunk) * 16 + byte);
-                const bf16x4 part = __builtin_bit_cast(
-                    bf16x4,
-                    __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(at)));
+            for (int p = 0; p < kPlanes<T>; ++p)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    a[4 * u + i] = part[i];
-            }
-            out[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, w.v[t], out[d], 0, 0, 0);
+                for (int u = 0; u < 2; ++u)
+                {
+                    const LdsBytes at =
+                        tile + (p * R + first_row + 16 * t + 8 * u) * L::kRowBytes
+                        + (L::kFlips ? base ^ (64 * d + 32 * u) // (rows 8 further on are moved by two chunks more)
+                                     : row * L::kRowBytes + L::place(16 * t + 8 * u + row, 4 * d + chunk) * 16 + byte);
+                    const bf16x4 part = __builtin_bit_cast(
+                        bf16x4,
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<__attribute__((address_space(3))) s16x4*>(at)));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        a[p][4 * u + i] = part[i];
+                }
+            multiply(a, w.v[t], &out[d]);
         }
-}
-template <int DP, bool Lean = false>
-__device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const Weights<float>& w, f32x16 (&out)[DP / 32])
-{
-    using L = Tile<float, DP>;
-    const int lane = threadIdx.x & (kWaveSize - 1);
-#pragma unroll
-    for (int i = 0; i < 16; ++i)
-    {
-        const int row = 8 * (i / 4) + i % 4 + 4 * (lane / 32);
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d)
-        {
-            const float a = *reinterpret_cast<__attribute__((address_space(3))) float*>(
-                tile + first_row * L::kRowBytes + L::address(row, 8 * d + (lane & 31) / 4) + (lane & 3) * 4);
-            out[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w.v[i], out[d], 0, 0, 0);
-        }
-    }
 }
 
 // Stores what accumulate() made of row l % 32 (v times factor), at p; Whole: rows begin on multiples of 16 bytes.

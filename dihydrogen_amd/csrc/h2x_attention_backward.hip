@@ -12,7 +12,7 @@ namespace attention
 namespace
 {
 
-// Rows of a tile that passes through LDS: 16 KB of 128 16-bit or 32-bit elements.
+// Rows of a tile that passes through LDS: 16 KB of 128 16-bit elements, 24 KB of floats.
 template <typename T>
 constexpr int kTileRows = sizeof(T) == 2 ? 64 : 32;
 
@@ -36,29 +36,13 @@ struct Args
     Schedule schedule;
 };
 
-// Sum of products of two fragments' elements, over both halves.
-template <typename T, int DP>
-__device__ __forceinline__ float dot(const Fragment<T, DP>& a, const Fragment<T, DP>& b)
-{
-    float sum = 0.0f;
-#pragma unroll
-    for (int c = 0; c < Tile<T, DP>::kChunks / 2; ++c)
-    {
-        const AVec<T, Tile<T, DP>::kPerChunk> x = __builtin_bit_cast(decltype(x), a.chunk[c]), y = __builtin_bit_cast(decltype(x), b.chunk[c]);
-#pragma unroll
-        for (int i = 0; i < Tile<T, DP>::kPerChunk; ++i)
-            sum = __builtin_fmaf(static_cast<float>(x.v[i]), static_cast<float>(y.v[i]), sum);
-    }
-    return halves_sum(sum);
-}
-
 // dq, and what the other pass needs of each row.  As in the forward pass, the waves of a workgroup take 32 queries of a head each.
 template <typename T, int DP, bool Whole>
 __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_dq_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
-    constexpr int KT = kTileRows<T>, kTileBytes = KT * Tile<T, DP>::kRowBytes;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
+    constexpr int KT = kTileRows<T>;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, KT>];
     const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks);
     if (place.head >= a.heads)
         return;
@@ -78,25 +62,42 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
     const T* const k = a.k + n * a.ks.sample + (head / a.group) * a.ks.head;
     const T* const v = a.v + n * a.vs.sample + (head / a.group) * a.vs.head;
     const int k_bytes = static_cast<int>(a.ks.token * sizeof(T)), v_bytes = static_cast<int>(a.vs.token * sizeof(T));
-    const auto load = [&](int tile) {
+    TileLoad<T, DP, KT, kThreads, Whole> k_load, v_load;
+    const auto issue = [&](int tile) {
         const int at = from + tile * KT, rows = min(KT, sample.keys - at);
-        load_tile<T, DP, KT, kThreads, Whole>(buffer_of(k + at * a.ks.token, rows, a.ks.token, a.dim), k_bytes, a.dim,
-                                              (LdsBytes) lds[tile & 1][0], threadIdx.x);
-        load_tile<T, DP, KT, kThreads, Whole>(buffer_of(v + at * a.vs.token, rows, a.vs.token, a.dim), v_bytes, a.dim,
-                                              (LdsBytes) lds[tile & 1][1], threadIdx.x);
+        k_load.issue(buffer_of(k + at * a.ks.token, rows, a.ks.token, a.dim), k_bytes, a.dim, (LdsBytes) lds[tile & 1][0],
+                     threadIdx.x);
+        v_load.issue(buffer_of(v + at * a.vs.token, rows, a.vs.token, a.dim), v_bytes, a.dim, (LdsBytes) lds[tile & 1][1],
+                     threadIdx.x);
+    };
+    const auto put = [&](int tile) {
+        k_load.put((LdsBytes) lds[tile & 1][0], threadIdx.x);
+        v_load.put((LdsBytes) lds[tile & 1][1], threadIdx.x);
     };
     if (tiles > 0)
-        load(0);
+    {
+        issue(0);
+        put(0);
+    }
 
     const bool there = i <= last;
     const int64_t row = (static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + i;
     Fragment<T, DP> q, d_o;
-    float delta, log2_sum = -kLowest;
+    float delta = 0.0f, log2_sum = -kLowest;
     {
-        Fragment<T, DP> o;
-        load_fragment<T, DP, Whole>(&o, a.o + n * a.os.sample + head * a.os.head + i * a.os.token, there, a.dim);
-        load_fragment<T, DP, Whole>(&d_o, a.d_o + n * a.d_os.sample + head * a.d_os.head + i * a.d_os.token, there, a.dim);
-        delta = dot<T, DP>(o, d_o);
+        const T* const o_row = a.o + n * a.os.sample + head * a.os.head + i * a.os.token;
+        const T* const d_o_row = a.d_o + n * a.d_os.sample + head * a.d_os.head + i * a.d_os.token;
+#pragma unroll
+        for (int c = 0; c < DP / 16; ++c)
+        {
+            const int at = 16 * c + 8 * (lane / 32);
+            const Eight<T> x = load_eight<T, Whole>(o_row, at, there, a.dim), y = load_eight<T, Whole>(d_o_row, at, there, a.dim);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                delta = __builtin_fmaf(element(x, e), element(y, e), delta);
+            planes_of(y, d_o.chunk[c]);
+        }
+        delta = halves_sum(delta);
     }
     load_fragment<T, DP, Whole>(&q, a.q + n * a.qs.sample + head * a.qs.head + i * a.qs.token, there, a.dim);
     if (there)
@@ -123,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
         wait_for_loads();
         __syncthreads();
         if (tile + 1 < tiles)
-            load(tile + 1);
+            issue(tile + 1);
         const LdsBytes k_tile = (LdsBytes) lds[tile & 1][0], v_tile = (LdsBytes) lds[tile & 1][1];
 #pragma unroll
         for (int b = 0; b < KT / 32; ++b)
@@ -132,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
             if (first > last || at >= some_end || at + 32 <= some_from)
                 continue;
             f32x16 s, dp;
-            two_products<T, DP>(k_tile, v_tile, 32 * b, q, d_o, &s, &dp);
+            two_products<T, DP, KT>(k_tile, v_tile, 32 * b, q, d_o, &s, &dp);
             if (at < all_from || at + 32 > all_end)
                 hide(&s, at, row_from, row_end);
             Weights<T> ds;
@@ -142,8 +143,10 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale_log2, -log2_sum));
                 ds.set(j, p * (dp[j] - delta));
             }
-            accumulate<DP>(k_tile, 32 * b, ds, dq);
+            accumulate<T, DP, KT>(k_tile, 32 * b, ds, dq);
         }
+        if (tile + 1 < tiles)
+            put(tile + 1); // (all waves are past the tile that lay there)
     }
     if (i < a.masks.queries)
         store_row<T, DP, Whole>(a.dq + n * a.dqs.sample + head * a.dqs.head + i * a.dqs.token, a.dim, dq, a.scale);
@@ -156,9 +159,8 @@ template <typename T, int DP, bool Whole>
 __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Whole>)) attention_dkv_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
-    constexpr bool kLean = false; // its rows leave no registers for addresses
-    constexpr int QT = kTileRows<T>, kTileBytes = QT * Tile<T, DP>::kRowBytes;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
+    constexpr int QT = kTileRows<T>;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, QT>];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kWaveSize];
     const int key_heads = a.query_heads / a.group;
     const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks);
@@ -178,15 +180,14 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
         tiles = (max(sample.end_query(block_end - 1) - from, 0) + QT - 1) / QT;
     }
     const int q_bytes = static_cast<int>(a.qs.token * sizeof(T)), d_o_bytes = static_cast<int>(a.d_os.token * sizeof(T));
+    TileLoad<T, DP, QT, kThreads, Whole> q_load, d_o_load;
     // tile `tile` of the group's head `g`, to stage `stage`
-    const auto load = [&](int g, int tile, int stage) {
+    const auto issue = [&](int g, int tile, int stage) {
         const int head = key_head * a.group + g, at = from + tile * QT, rows = min(QT, sample.queries - at);
         const T* const q = a.q + n * a.qs.sample + head * a.qs.head + at * a.qs.token;
         const T* const d_o = a.d_o + n * a.d_os.sample + head * a.d_os.head + at * a.d_os.token;
-        load_tile<T, DP, QT, kThreads, Whole>(buffer_of(q, rows, a.qs.token, a.dim), q_bytes, a.dim, (LdsBytes) lds[stage][0],
-                                              threadIdx.x);
-        load_tile<T, DP, QT, kThreads, Whole>(buffer_of(d_o, rows, a.d_os.token, a.dim), d_o_bytes, a.dim, (LdsBytes) lds[stage][1],
-                                              threadIdx.x);
+        q_load.issue(buffer_of(q, rows, a.qs.token, a.dim), q_bytes, a.dim, (LdsBytes) lds[stage][0], threadIdx.x);
+        d_o_load.issue(buffer_of(d_o, rows, a.d_os.token, a.dim), d_o_bytes, a.dim, (LdsBytes) lds[stage][1], threadIdx.x);
         // rows' logarithms by one wave, their deltas by another (zero behind the sample's queries, as q and d_o are)
         if (wave < 2)
         {
@@ -195,9 +196,16 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
             load_numbers(buffer_of(p, rows, 1, 1), (LdsBytes) stats[stage][wave], lane);
         }
     };
+    const auto put = [&](int stage) {
+        q_load.put((LdsBytes) lds[stage][0], threadIdx.x);
+        d_o_load.put((LdsBytes) lds[stage][1], threadIdx.x);
+    };
     const int steps = tiles * a.group;
     if (steps > 0)
-        load(0, 0, 0);
+    {
+        issue(0, 0, 0);
+        put(0);
+    }
 
     const bool there = j <= last;
     Fragment<T, DP> k, v;
@@ -220,7 +228,7 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
         if (++tile == tiles)
             tile = 0, ++g;
         if (step + 1 < steps)
-            load(g, tile, stage ^ 1);
+            issue(g, tile, stage ^ 1);
         const LdsBytes q_tile = (LdsBytes) lds[stage][0], d_o_tile = (LdsBytes) lds[stage][1];
 #pragma unroll
         for (int b = 0; b < QT / 32; ++b)
@@ -231,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
             const float* const log2_sum = &stats[stage][0][32 * b + 4 * (lane / 32)];
             const float* const delta = &stats[stage][1][32 * b + 4 * (lane / 32)];
             Weights<T> p, ds;
-            f32x16 s = product<T, DP, kLean>(q_tile, 32 * b, k);
+            f32x16 s = product<T, DP, QT>(q_tile, 32 * b, k);
             if (at < all_from || at + 32 > all_end)
                 hide(&s, at, row_from, row_end);
 #pragma unroll
@@ -245,8 +253,8 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
                     p.set(r + e, s[r + e]);
                 }
             }
-            accumulate<DP, kLean>(d_o_tile, 32 * b, p, dv);
-            const f32x16 dp = product<T, DP, kLean>(d_o_tile, 32 * b, v);
+            accumulate<T, DP, QT>(d_o_tile, 32 * b, p, dv);
+            const f32x16 dp = product<T, DP, QT>(d_o_tile, 32 * b, v);
 #pragma unroll
             for (int r = 0; r < 16; r += 4)
             {
@@ -255,8 +263,10 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
                 for (int e = 0; e < 4; ++e)
                     ds.set(r + e, s[r + e] * (dp[r + e] - l[e]));
             }
-            accumulate<DP, kLean>(q_tile, 32 * b, ds, dk);
+            accumulate<T, DP, QT>(q_tile, 32 * b, ds, dk);
         }
+        if (step + 1 < steps)
+            put(stage ^ 1);
     }
     if (j < a.masks.keys)
     {

@@ -11,7 +11,7 @@ namespace attention
 namespace
 {
 
-// Keys of a tile: 16 KB of 128 16-bit or 32-bit elements.
+// Keys of a tile: 16 KB of 128 16-bit elements, 24 KB of floats.
 template <typename T>
 constexpr int kTileKeys = sizeof(T) == 2 ? 64 : 32;
 
@@ -34,7 +34,7 @@ struct Args
     Parts parts;
     float scale_log2;
     int dim, samples, query_heads, group, query_blocks;
-    int heads; // of all samples; few queries: key heads
+    int heads; // of all samples; with split keys key heads
     Schedule schedule;
 };
 
@@ -59,7 +59,7 @@ struct Rows32
     // The scores of a tile's keys.
     __device__ __forceinline__ void score(LdsBytes k_tile, f32x16 (&s)[kTileKeys<T> / 32]) const
     {
-        products<T, DP>(k_tile, 0, q, s);
+        products<T, DP, kTileKeys<T>>(k_tile, 0, q, s);
     }
 
     // Scores to probabilities, with maximum, sum and output brought up to date.
@@ -110,46 +110,22 @@ struct Rows32
     {
 #pragma unroll
         for (int b = 0; b < kTileKeys<T> / 32; ++b)
-            accumulate<DP>(v_tile, 32 * b, w[b], out);
+            accumulate<T, DP, kTileKeys<T>>(v_tile, 32 * b, w[b], out);
     }
 };
-
-// Writes row `row` of the outputs (whose element 0 lies at o): what is there is out / sum, or a part's share.  max, sum: of the whole row.
-template <typename T, int DP, bool Whole>
-__device__ __forceinline__ void finish_row(const Args<T>& a, T* o, int64_t row, int part, const f32x16 (&out)[DP / 32],
-                                           float max, float sum)
-{
-    const bool first_half = (threadIdx.x & 32) == 0;
-    if (a.parts.num == 1)
-    {
-        store_row<T, DP, Whole>(o, a.dim, out, sum > 0.0f ? 1.0f / sum : 0.0f);
-        if (a.logsumexp && first_half)
-            a.logsumexp[row] = sum > 0.0f ? (max + log2f(sum)) * kLn2 : -INFINITY;
-        return;
-    }
-    const int64_t rows = static_cast<int64_t>(a.samples) * a.query_heads * a.masks.queries, at = part * rows + row;
-    if (first_half)
-    {
-        a.parts.max_sum[2 * at] = max;
-        a.parts.max_sum[2 * at + 1] = sum;
-    }
-    if (sum > 0.0f)
-        store_row<float, DP, true>(a.parts.out + at * DP, DP, out, 1.0f);
-}
 
 // Many queries: the waves of a workgroup take 32 queries of a head each, and share the tiles of keys and values, which come
 // straight from memory to LDS while the tile before them is worked on.
 template <typename T, int DP, bool Whole>
-__global__ void __launch_bounds__(kThreads, 2) attention_forward_kernel(const Args<T> a)
+__global__ void __launch_bounds__(kThreads, (sizeof(T) == 2 || DP <= 96 ? 2 : 1)) attention_forward_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
-    constexpr int KT = kTileKeys<T>, kTileBytes = KT * Tile<T, DP>::kRowBytes;
-    __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes];
-    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.query_blocks * a.parts.num);
+    constexpr int KT = kTileKeys<T>;
+    __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, KT>];
+    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.query_blocks);
     if (place.head >= a.heads)
         return;
-    const int block = place.block / a.parts.num, part = place.block - block * a.parts.num;
-    const int n = place.head / a.query_heads, head = place.head - n * a.query_heads;
+    const int block = place.block, n = place.head / a.query_heads, head = place.head - n * a.query_heads;
     const int lane = threadIdx.x & (kWaveSize - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const Sample sample = sample_of(a.masks, n);
 
@@ -163,21 +139,26 @@ __global__ void __launch_bounds__(kThreads, 2) attention_forward_kernel(const Ar
         from = sample.first_key(block_first);
         tiles = (max(sample.end_key(block_end - 1) - from, 0) + KT - 1) / KT;
     }
-    const int first_tile = static_cast<int>(static_cast<int64_t>(tiles) * part / a.parts.num);
-    const int end_tile = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / a.parts.num);
-
     const T* const k = a.k + n * a.ks.sample + (head / a.group) * a.ks.head;
     const T* const v = a.v + n * a.vs.sample + (head / a.group) * a.vs.head;
     const int k_bytes = static_cast<int>(a.ks.token * sizeof(T)), v_bytes = static_cast<int>(a.vs.token * sizeof(T));
-    const auto load = [&](int tile) {
+    TileLoad<T, DP, KT, kThreads, Whole> k_load, v_load;
+    const auto issue = [&](int tile) {
         const int at = from + tile * KT, rows = min(KT, sample.keys - at);
-        load_tile<T, DP, KT, kThreads, Whole>(buffer_of(k + at * a.ks.token, rows, a.ks.token, a.dim), k_bytes, a.dim,
-                                              (LdsBytes) lds[tile & 1][0], threadIdx.x);
-        load_tile<T, DP, KT, kThreads, Whole>(buffer_of(v + at * a.vs.token, rows, a.vs.token, a.dim), v_bytes, a.dim,
-                                              (LdsBytes) lds[tile & 1][1], threadIdx.x);
+        k_load.issue(buffer_of(k + at * a.ks.token, rows, a.ks.token, a.dim), k_bytes, a.dim, (LdsBytes) lds[tile & 1][0],
+                     threadIdx.x);
+        v_load.issue(buffer_of(v + at * a.vs.token, rows, a.vs.token, a.dim), v_bytes, a.dim, (LdsBytes) lds[tile & 1][1],
+                     threadIdx.x);
     };
-    if (first_tile < end_tile)
-        load(first_tile);
+    const auto put = [&](int tile) {
+        k_load.put((LdsBytes) lds[tile & 1][0], threadIdx.x);
+        v_load.put((LdsBytes) lds[tile & 1][1], threadIdx.x);
+    };
+    if (tiles > 0)
+    {
+        issue(0);
+        put(0);
+    }
 
     Rows32<T, DP> rows;
     rows.clear();
@@ -188,12 +169,12 @@ __global__ void __launch_bounds__(kThreads, 2) attention_forward_kernel(const Ar
     const int some_from = sample.first_key(first), some_end = sample.end_key(last);
     const int all_from = sample.first_key(last), all_end = sample.end_key(first);
 
-    for (int tile = first_tile; tile < end_tile; ++tile)
+    for (int tile = 0; tile < tiles; ++tile)
     {
         wait_for_loads();
         __syncthreads();
-        if (tile + 1 < end_tile)
-            load(tile + 1);
+        if (tile + 1 < tiles)
+            issue(tile + 1);
         const int at = from + tile * KT;
         if (first <= last && at < some_end && at + KT > some_from)
         {
@@ -203,32 +184,37 @@ __global__ void __launch_bounds__(kThreads, 2) attention_forward_kernel(const Ar
             rows.soften(s, w, at, at < all_from || at + KT > all_end, a.scale_log2);
             rows.weigh((LdsBytes) lds[tile & 1][1], w);
         }
+        if (tile + 1 < tiles)
+            put(tile + 1); // (all waves are past the tile that lay there)
     }
     if (i < a.masks.queries)
     {
         const bool there = i < sample.queries;
         const float sum = halves_sum(rows.sum);
-        finish_row<T, DP, Whole>(a, a.o + n * a.os.sample + head * a.os.head + i * a.os.token,
-                                 (static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + i, part, rows.out, rows.max,
-                                 there ? sum : 0.0f);
+        store_row<T, DP, Whole>(a.o + n * a.os.sample + head * a.os.head + i * a.os.token, a.dim, rows.out,
+                                there && sum > 0.0f ? 1.0f / sum : 0.0f);
+        if (a.logsumexp && lane < 32)
+            a.logsumexp[(static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + i] =
+                there && sum > 0.0f ? (rows.max + log2f(sum)) * kLn2 : -INFINITY;
     }
 #endif
 }
 
-// Few queries: the queries of all heads that share a key head are rows of one wave's tile, so that keys and values are read once.
-// The waves of a workgroup go through different tiles of the same part of the keys, each with LDS of its own and without barriers, and join what
-// they have at the end.
+// Few workgroups' worth of queries: the queries of all heads that share a key head are rows one after another, 32 of them a workgroup, so
+// that keys and values are read once for them.  The waves of a workgroup go through different tiles of the same part of the keys,
+// each with LDS of its own and without barriers, and join what they have at the end.
 template <typename T, int DP, bool Whole>
-__global__ void __launch_bounds__(kThreads) attention_few_kernel(const Args<T> a)
+__global__ void __launch_bounds__(kThreads) attention_split_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
-    constexpr int KT = kTileKeys<T>, kTileBytes = KT * Tile<T, DP>::kRowBytes;
-    constexpr int kLoads = KT * Tile<T, DP>::kChunks / kWaveSize; // of a wave, for a tile
-    constexpr int kJoinStride = DP + 4;
-    constexpr int kJoinBytes = kWaves * kRows * kJoinStride * 4, kTilesBytes = kWaves * 2 * kTileBytes;
+    constexpr int KT = kTileKeys<T>;
+    using Load = TileLoad<T, DP, KT, kWaveSize, Whole>;
+    // Tiles that go straight to LDS have a place for keys and one for values; those that pass through registers take turns at one.
+    constexpr int kBytes = kTileBytes<T, DP, KT>, kTilesBytes = kWaves * (Load::kDirect ? 2 : 1) * kBytes;
+    constexpr int kJoinStride = DP + 4, kJoinBytes = kWaves * kRows * kJoinStride * 4;
     __shared__ __attribute__((aligned(16))) char lds[kTilesBytes > kJoinBytes ? kTilesBytes : kJoinBytes];
     __shared__ float max_sum[kWaves][kRows][2];
-    const Place place = place_of({kByHead, 0}, blockIdx.x, gridDim.x, a.heads, a.query_blocks * a.parts.num);
+    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.query_blocks * a.parts.num);
     if (place.head >= a.heads)
         return;
     const int key_heads = a.query_heads / a.group;
@@ -255,11 +241,12 @@ __global__ void __launch_bounds__(kThreads) attention_few_kernel(const Args<T> a
 
     const T* const k = a.k + n * a.ks.sample + key_head * a.ks.head;
     const T* const v = a.v + n * a.vs.sample + key_head * a.vs.head;
-    const LdsBytes k_tile = (LdsBytes) (lds + wave * 2 * kTileBytes), v_tile = k_tile + kTileBytes;
-    const auto load = [&](const T* p, const Strides& s, int tile, LdsBytes to) {
+    const LdsBytes k_tile = (LdsBytes) (lds + wave * (Load::kDirect ? 2 : 1) * kBytes), v_tile = k_tile + (Load::kDirect ? kBytes : 0);
+    Load k_load, v_load;
+    const auto issue = [&](Load* load, const T* p, const Strides& s, int tile, LdsBytes to) {
         const int at = from + tile * KT;
-        load_tile<T, DP, KT, kWaveSize, Whole>(buffer_of(p + at * s.token, min(KT, sample.keys - at), s.token, a.dim),
-                                               static_cast<int>(s.token * sizeof(T)), a.dim, to, lane);
+        load->issue(buffer_of(p + at * s.token, min(KT, sample.keys - at), s.token, a.dim), static_cast<int>(s.token * sizeof(T)),
+                    a.dim, to, lane);
     };
 
     Rows32<T, DP> rows;
@@ -273,35 +260,36 @@ __global__ void __launch_bounds__(kThreads) attention_few_kernel(const Args<T> a
     int tile = first_tile + wave;
     if (tile < end_tile)
     {
-        load(k, a.ks, tile, k_tile);
-        load(v, a.vs, tile, v_tile);
+        issue(&k_load, k, a.ks, tile, k_tile);
+        issue(&v_load, v, a.vs, tile, v_tile);
     }
     for (; tile < end_tile; tile += kWaves)
     {
         const int at = from + tile * KT;
         f32x16 s[KT / 32];
         Weights<T> w[KT / 32];
-        if constexpr (Whole)
-            wait_for_loads<kLoads>(); // the keys are there, the values may be under way
-        else
-            wait_for_lds();
+        if constexpr (Load::kDirect)
+            wait_for_loads<Load::kEach>(); // the keys are there, the values may be under way
+        k_load.put(k_tile, lane);
         rows.score(k_tile, s);
         wait_for_lds();
         const bool more = tile + kWaves < end_tile;
         if (more)
-            load(k, a.ks, tile + kWaves, k_tile);
+            issue(&k_load, k, a.ks, tile + kWaves, k_tile);
         // (a row beyond the sample's queries sees no key, and its wave no tile as a whole)
         rows.soften(s, w, at, at < all_from || at + KT > all_end, a.scale_log2);
-        if constexpr (!Whole)
-            wait_for_lds();
-        else if (more)
-            wait_for_loads<kLoads>();
-        else
-            wait_for_loads<0>();
+        if constexpr (Load::kDirect)
+        {
+            if (more)
+                wait_for_loads<Load::kEach>();
+            else
+                wait_for_loads<0>();
+        }
+        v_load.put(v_tile, lane);
         rows.weigh(v_tile, w);
         wait_for_lds();
         if (more)
-            load(v, a.vs, tile + kWaves, v_tile);
+            issue(&v_load, v, a.vs, tile + kWaves, v_tile);
     }
 
     // the waves' shares to LDS, and joined: thread t takes row t % 32 and every eighth run of four elements
@@ -373,16 +361,17 @@ __global__ void __launch_bounds__(kThreads) attention_few_kernel(const Args<T> a
 #endif
 }
 
-// Joins the parts of a row, a workgroup a row: a lane has a part's maximum and sum, a wave every fourth part's output.  (With a wave a row, one
-// part after another, 512 rows of 16 parts took 21 us: a chain of waits for memory.)
+// Joins the parts of a row: a lane has a part's maximum and sum, and S waves (one or four) take every S-th part's output.  (With one wave a
+// row, one part after another, 512 rows of 16 parts took 21 us, a chain of waits for memory; with four 16016 rows of two parts 19.)
 constexpr int kMostParts = kWaveSize;
-template <typename T, int DP>
+template <typename T, int DP, int S>
 __global__ void __launch_bounds__(kThreads) attention_join_kernel(const Args<T> a)
 {
     constexpr int N = (DP + kWaveSize - 1) / kWaveSize; // elements of a lane
-    __shared__ float outs[kWaves][N * kWaveSize], factors[kMostParts];
-    const int64_t rows = static_cast<int64_t>(a.samples) * a.query_heads * a.masks.queries, row = blockIdx.x;
+    __shared__ float outs[kWaves][N * kWaveSize], factors[kWaves][kMostParts];
     const int lane = threadIdx.x & (kWaveSize - 1), wave = threadIdx.x / kWaveSize;
+    const int64_t rows = static_cast<int64_t>(a.samples) * a.query_heads * a.masks.queries;
+    const int64_t row = min(static_cast<int64_t>(blockIdx.x) * (kWaves / S) + wave / S, rows - 1); // (the last one more than once)
     float max = kLowest, sum = 0.0f;
     if (lane < a.parts.num)
     {
@@ -392,15 +381,14 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const Args<T> 
     const bool any = sum > 0.0f; // (where no key was seen the output was not written)
     const float most = wave_combine(any ? max : kLowest, [](float x, float y) { return fmaxf(x, y); });
     const float factor = any ? __builtin_amdgcn_exp2f(max - most) : 0.0f;
-    if (wave == 0)
-        factors[lane] = factor;
+    factors[wave][lane] = factor;
     sum = token::wave_total(sum * factor);
     __syncthreads();
     float out[N] = {};
 #pragma unroll 4
-    for (int p = wave; p < a.parts.num; p += kWaves)
+    for (int p = wave % S; p < a.parts.num; p += S)
     {
-        const float f = factors[p];
+        const float f = factors[wave][p];
 #pragma unroll
         for (int n = 0; n < N; ++n)
         {
@@ -408,17 +396,28 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const Args<T> 
             out[n] = f > 0.0f ? __builtin_fmaf(x, f, out[n]) : out[n];
         }
     }
+    if constexpr (S > 1)
+    {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-        outs[wave][n * kWaveSize + lane] = out[n];
-    __syncthreads();
-    const int d = threadIdx.x;
+        for (int n = 0; n < N; ++n)
+            outs[wave][n * kWaveSize + lane] = out[n];
+        __syncthreads();
+        if (wave > 0)
+            return;
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int w = 1; w < S; ++w)
+                out[n] += outs[w][n * kWaveSize + lane];
+    }
     const int64_t of_head = row / a.masks.queries, i = row - of_head * a.masks.queries;
     const int64_t n = of_head / a.query_heads, head = of_head - n * a.query_heads;
     T* const o = a.o + n * a.os.sample + head * a.os.head + i * a.os.token;
-    if (d < a.dim)
-        o[d] = static_cast<T>(sum > 0.0f ? (outs[0][d] + outs[1][d] + outs[2][d] + outs[3][d]) / sum : 0.0f);
-    if (a.logsumexp && d == 0)
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+        if (e * kWaveSize + lane < a.dim)
+            o[e * kWaveSize + lane] = static_cast<T>(sum > 0.0f ? out[e] / sum : 0.0f);
+    if (a.logsumexp && lane == 0)
         a.logsumexp[row] = sum > 0.0f ? (most + log2f(sum)) * kLn2 : -INFINITY;
 }
 
@@ -427,7 +426,7 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const Args<T> 
 // How a call is run.
 struct Plan
 {
-    bool few;
+    bool split; // the keys among the waves of a workgroup
     int query_blocks, parts, padded_dim;
     uint64_t groups; // workgroups
 };
@@ -435,21 +434,29 @@ struct Plan
 Plan plan_of(const h2x_attention& a)
 {
     Plan p{};
-    const int64_t group = a.query_heads / a.key_heads;
-    p.few = a.queries <= 16;
+    const int64_t units = chip_units(), group = a.query_heads / a.key_heads;
+    const int64_t wide_blocks = (a.queries + kWaves * kRows - 1) / (kWaves * kRows), wide = wide_blocks * a.samples * a.query_heads;
+    const int64_t blocks = (group * a.queries + kRows - 1) / kRows, groups = blocks * a.samples * a.key_heads;
+    // Workgroups of 128 queries where there are enough of them: from half a workgroup for each CU on, or where the keys are a tile or two.  (us,
+    // 128 queries against split keys, bf16 unless said: 24 such workgroups, 196 keys, 8.8 and 7.5; 80, 577 keys, 13.4 and 11.6; 128, 2048
+    // keys, 43.9 and 42.9, causal 41.8 and 30.5; floats, 1001 keys, causal, 82 and 50; 240, 577 keys, 18 and 42; 256, 2048 keys, 48 and 81;
+    // 64 and 128, 128 and 64 keys, 6.7 and 7.2, 5.1 and 7.4.)
+    p.split = a.queries <= 16 || (2 * wide <= units && a.keys > 128);
     p.padded_dim = (a.head_dim + 31) / 32 * 32;
-    const int64_t blocks = p.few ? (group * a.queries + kRows - 1) / kRows : (a.queries + kWaves * kRows - 1) / (kWaves * kRows);
-    const int64_t groups = static_cast<int64_t>(a.samples) * (p.few ? a.key_heads : a.query_heads) * blocks;
-    // The keys in parts while there are not workgroups for each CU several times, a part being eight tiles at least for each of
-    // the waves that go through it one by one, or for the workgroup.
-    const int tile = a.dtype == H2X_F32 ? 32 : 64;
-    const int64_t least = p.few ? 4 * kWaves * tile : 8 * tile, aim = (p.few ? 8 : 2) * static_cast<int64_t>(chip_units());
-    int64_t parts = 1;
-    while (parts < kMostParts && groups * parts < aim && a.keys >= 2 * parts * least)
-        parts *= 2;
-    p.query_blocks = static_cast<int>(blocks);
-    p.parts = static_cast<int>(parts);
-    p.groups = static_cast<uint64_t>(groups) * parts;
+    p.query_blocks = static_cast<int>(p.split ? blocks : wide_blocks);
+    p.parts = 1;
+    if (p.split)
+    {
+        // The keys in parts too while that makes no more workgroups than run at once (twice as many where they are of unlike lengths), 512 keys a
+        // part at least; two parts are worth the joining from 4096 keys on.  (us for 1, 2, 4 ... 64 parts: 8 workgroups, 16384 keys of 128, 118,
+        // 67, 40, 27, 22, 24, 36; 128 workgroups, 16384 keys, 213, 191, 194, 205; 2048 keys, 27, 30, 35.)
+        const bool unlike = a.queries > 16 && (a.window_left < 0) != (a.window_right < 0);
+        while (p.parts < kMostParts && groups * p.parts * 2 <= (unlike ? 2 : 1) * units && a.keys >= 1024 * static_cast<int64_t>(p.parts))
+            p.parts *= 2;
+        if (p.parts == 2 && a.keys < 4096 && !unlike)
+            p.parts = 1;
+    }
+    p.groups = static_cast<uint64_t>(p.split ? groups : wide) * p.parts;
     return p;
 }
 
@@ -470,12 +477,15 @@ int issue(const h2x_attention& c, const Plan& p, const Args<T>& a, hipStream_t s
     const dim3 grid(static_cast<uint32_t>((p.groups + kNumXcd - 1) / kNumXcd * kNumXcd));
     return with_padded_dim(c.head_dim, [&](auto dim) {
         constexpr int DP = decltype(dim)::value;
-        if (p.few)
-            launch(attention_few_kernel<T, DP, Whole>, grid, dim3(kThreads), stream, a);
+        if (p.split)
+            launch(attention_split_kernel<T, DP, Whole>, grid, dim3(kThreads), stream, a);
         else
             launch(attention_forward_kernel<T, DP, Whole>, grid, dim3(kThreads), stream, a);
-        if (p.parts > 1)
-            launch(attention_join_kernel<T, DP>, dim3(static_cast<uint32_t>(rows_of(c))), dim3(kThreads), stream, a);
+        if (p.parts > 4)
+            launch(attention_join_kernel<T, DP, 4>, dim3(static_cast<uint32_t>(rows_of(c))), dim3(kThreads), stream, a);
+        else if (p.parts > 1)
+            launch(attention_join_kernel<T, DP, 1>, dim3(static_cast<uint32_t>((rows_of(c) + kWaves - 1) / kWaves)), dim3(kThreads),
+                   stream, a);
         return launch_status();
     });
 }
@@ -539,7 +549,7 @@ extern "C" int h2x_attention_forward(const h2x_attention* attention, const void*
         a.query_heads = c.query_heads;
         a.group = c.query_heads / c.key_heads;
         a.query_blocks = p.query_blocks;
-        a.heads = c.samples * (p.few ? c.key_heads : c.query_heads);
+        a.heads = c.samples * (p.split ? c.key_heads : c.query_heads);
         a.schedule = schedule_of(c, false, a.heads, static_cast<uint64_t>(p.query_blocks) * p.parts);
         return issue<T, decltype(is_whole)::value>(c, p, a, as_stream(stream));
     });
