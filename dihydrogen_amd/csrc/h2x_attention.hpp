@@ -109,6 +109,8 @@ __device__ __forceinline__ Place place_of(const Schedule& s, uint32_t id, uint32
     return {static_cast<int>(head), static_cast<int>(s.order == kFirstFirst ? block : blocks - 1 - block)};
 }
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -141,14 +143,19 @@ __device__ __forceinline__ float halves_sum(float v)
 template <typename T>
 constexpr int kPlanes = sizeof(T) == 2 ? 1 : 3; // 16-bit numbers of an element
 
-// x as a sum of 16-bit numbers, largest first.
-__device__ __forceinline__ void split(float x, bf16 (&v)[3])
+// x and y as sums of 16-bit numbers, largest first, two numbers to a word as they lie in memory.
+__device__ __forceinline__ void split(float x, float y, uint32_t (&v)[3])
 {
-    v[0] = static_cast<bf16>(x);
-    x -= static_cast<float>(v[0]);
-    v[1] = static_cast<bf16>(x);
-    x -= static_cast<float>(v[1]);
-    v[2] = static_cast<bf16>(x);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+    {
+        v[p] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
+        if (p < 2)
+        {
+            x -= __uint_as_float(v[p] << 16);
+            y -= __uint_as_float(v[p] & 0xffff0000u);
+        }
+    }
 }
 
 // Eight neighbouring elements as they come from memory.
@@ -170,15 +177,19 @@ __device__ __forceinline__ void planes_of(const Eight<bf16>& e, bf16x8 (&out)[1]
 }
 __device__ __forceinline__ void planes_of(const Eight<float>& e, bf16x8 (&out)[3])
 {
+    u32x4 words[3];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
     {
-        bf16 parts[3];
-        split(__uint_as_float(e.v[i / 4][i % 4]), parts);
-        out[0][i] = parts[0];
-        out[1][i] = parts[1];
-        out[2][i] = parts[2];
+        uint32_t parts[3];
+        split(__uint_as_float(e.v[i / 2][i % 2 * 2]), __uint_as_float(e.v[i / 2][i % 2 * 2 + 1]), parts);
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+            words[p][i] = parts[p];
     }
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+        out[p] = __builtin_bit_cast(bf16x8, words[p]);
 }
 __device__ __forceinline__ float element(const Eight<bf16>& e, int i)
 {
@@ -461,19 +472,26 @@ __device__ __forceinline__ void two_products(LdsBytes tile_s, LdsBytes tile_t, i
 template <typename T>
 struct Weights
 {
-    bf16x8 v[2][kPlanes<T>];
-    __device__ __forceinline__ void set(int i, float x)
+    u32x4 words[2][kPlanes<T>];
+    // Numbers i (even) and i + 1 of the lane.
+    __device__ __forceinline__ void set(int i, float x, float y)
     {
         if constexpr (kPlanes<T> == 1)
-            v[i / 8][0][i % 8] = static_cast<bf16>(x);
+            words[i / 8][0][i % 8 / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{x, y}), bf16x2));
         else
         {
-            bf16 parts[3];
-            split(x, parts);
+            uint32_t parts[3];
+            split(x, y, parts);
 #pragma unroll
             for (int p = 0; p < 3; ++p)
-                v[i / 8][p][i % 8] = parts[p];
+                words[i / 8][p][i % 8 / 2] = parts[p];
         }
+    }
+    __device__ __forceinline__ void operand(int t, bf16x8 (&v)[kPlanes<T>]) const
+    {
+#pragma unroll
+        for (int p = 0; p < kPlanes<T>; ++p)
+            v[p] = __builtin_bit_cast(bf16x8, words[t][p]);
     }
 };
 
@@ -493,7 +511,8 @@ __device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const W
 #pragma unroll
         for (int t = 0; t < 2; ++t)
         {
-            bf16x8 a[kPlanes<T>];
+            bf16x8 a[kPlanes<T>], b[kPlanes<T>];
+            w.operand(t, b);
 #pragma unroll
             for (int p = 0; p < kPlanes<T>; ++p)
 #pragma unroll
@@ -510,7 +529,7 @@ __device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const W
                     for (int i = 0; i < 4; ++i)
                         a[p][4 * u + i] = part[i];
                 }
-            multiply(a, w.v[t], &out[d]);
+            multiply(a, b, &out[d]);
         }
 }
 

@@ -139,10 +139,10 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
             Weights<T> ds;
 #pragma unroll
             for (int j = 0; j < 16; ++j)
-            {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale_log2, -log2_sum));
-                ds.set(j, p * (dp[j] - delta));
-            }
+                s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale_log2, -log2_sum)) * (dp[j] - delta);
+#pragma unroll
+            for (int j = 0; j < 16; j += 2)
+                ds.set(j, s[j], s[j + 1]);
             accumulate<T, DP, KT>(k_tile, 32 * b, ds, dq);
         }
         if (tile + 1 < tiles)
@@ -248,10 +248,9 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
                 const f32x4 l = *reinterpret_cast<const f32x4*>(log2_sum + 2 * r);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                {
                     s[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + e], a.scale_log2, -l[e]));
-                    p.set(r + e, s[r + e]);
-                }
+                p.set(r, s[r], s[r + 1]);
+                p.set(r + 2, s[r + 2], s[r + 3]);
             }
             accumulate<T, DP, QT>(d_o_tile, 32 * b, p, dv);
             const f32x16 dp = product<T, DP, QT>(d_o_tile, 32 * b, v);
@@ -261,7 +260,9 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
                 const f32x4 l = *reinterpret_cast<const f32x4*>(delta + 2 * r);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    ds.set(r + e, s[r + e] * (dp[r + e] - l[e]));
+                    s[r + e] *= dp[r + e] - l[e];
+                ds.set(r, s[r], s[r + 1]);
+                ds.set(r + 2, s[r + 2], s[r + 3]);
             }
             accumulate<T, DP, QT>(q_tile, 32 * b, ds, dk);
         }

@@ -97,11 +97,13 @@ struct Rows32
 #pragma unroll
         for (int b = 0; b < B; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 16; i += 2)
             {
                 const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], scale_log2, -max));
+                const float q = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i + 1], scale_log2, -max));
                 part += p;
-                w[b].set(i, p);
+                part += q;
+                w[b].set(i, p, q);
             }
         sum += part;
     }
