@@ -20,6 +20,24 @@ constexpr int kTileRows = sizeof(T) == 2 ? 64 : 32;
 template <typename T, int DP, bool Whole>
 constexpr int kWavesOf = Whole && (sizeof(T) == 2 || DP <= 64) ? 2 : 1;
 
+// With one wave a SIMD half of a lane's 512 registers are the matrix units' own: sums stay there from tile to tile.  (Left to itself the compiler
+// moves all of them to and fro at each: 190 instructions of 700 for floats, heads of 96.)
+template <int D>
+__device__ __forceinline__ void keep_apart(f32x16 (&v)[D])
+{
+#ifdef __HIP_DEVICE_COMPILE__
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+        asm volatile("" : "+a"(v[d]));
+#endif
+}
+template <int D>
+__device__ __forceinline__ void keep_apart(f32x16 (&v)[D], f32x16 (&w)[D])
+{
+    keep_apart(v);
+    keep_apart(w);
+}
+
 template <typename T>
 struct Args
 {
@@ -147,6 +165,8 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
         }
         if (tile + 1 < tiles)
             put(tile + 1); // (all waves are past the tile that lay there)
+        if constexpr (kWavesOf<T, DP, Whole> == 1)
+            keep_apart(dq);
     }
     if (i < a.masks.queries)
         store_row<T, DP, Whole>(a.dq + n * a.dqs.sample + head * a.dqs.head + i * a.dqs.token, a.dim, dq, a.scale);
@@ -159,6 +179,7 @@ template <typename T, int DP, bool Whole>
 __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Whole>)) attention_dkv_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
+    constexpr bool kOneWave = DP == 128 || kWavesOf<T, DP, Whole> == 1; // (128 elements: two waves would have to spill)
     constexpr int QT = kTileRows<T>;
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, QT>];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kWaveSize];
@@ -268,6 +289,8 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
         }
         if (step + 1 < steps)
             put(stage ^ 1);
+        if constexpr (kOneWave)
+            keep_apart(dk, dv);
     }
     if (j < a.masks.keys)
     {
