@@ -271,20 +271,45 @@ struct Tile
 template <typename T, int DP, int R>
 constexpr int kTileBytes = kPlanes<T>* R* Tile<DP>::kRowBytes;
 
-// A buffer of `rows` rows of `dim` elements, `stride` elements apart: reads behind it give zero.
+// A buffer of `rows` rows of `dim` elements, `stride` elements apart: reads behind it give zero.  (The words of a buffer descriptor, the same in all
+// lanes.)
 template <typename T>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const T* p, int rows, int64_t stride, int dim)
+__device__ __forceinline__ u32x4 buffer_of(const T* p, int rows, int64_t stride, int dim)
 {
     const int64_t bytes = rows > 0 ? ((rows - 1) * stride + dim) * static_cast<int64_t>(sizeof(T)) : 0;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), 0, static_cast<int>(bytes), 0x00020000);
+    const uint64_t base = reinterpret_cast<uint64_t>(p);
+    return {static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(base))),
+            static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(base >> 32 & 0xffff))),
+            static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(bytes))), 0x00020000u};
+}
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t resource_of(const u32x4& b)
+{
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(static_cast<uint64_t>(b[1]) << 32 | b[0]), 0, static_cast<int>(b[2]),
+                                             static_cast<int>(b[3]));
 }
 constexpr unsigned int kOutside = 0x80000000u; // behind every buffer
+
+// 16 or 4 bytes a lane from a buffer straight to LDS, to `to` (the same in all lanes) and on.  In assembly, because the compiler waits for
+// all loads that its own form of these has issued before it reads any LDS across, those for the next tile among them (gradients of keys,
+// heads of 128: 674 us, 550 without loads).  Nothing is returned to registers; who reads the LDS waits with wait_for_loads().  (Five wait states
+// between a lane's number put into a scalar register and a load that uses it, one after m0: the compiler does not see to that in assembly.)
+template <int Bytes>
+__device__ __forceinline__ void load_to_lds(const u32x4& b, unsigned int at, LdsBytes to)
+{
+    const int place = __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>(to)));
+    if constexpr (Bytes == 16)
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(place), "v"(at), "s"(b) : "memory");
+    else
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(place), "v"(at), "s"(b) : "memory");
+}
 
 // Until no more than N of this wave's loads are under way (they arrive in order).
 template <int N = 0>
 __device__ __forceinline__ void wait_for_loads()
 {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | N >> 4 << 14); // (an instruction that the compiler counts with)
+    asm volatile("" ::: "memory");
 }
 // Until what this wave has asked of LDS is there.
 __device__ __forceinline__ void wait_for_lds()
@@ -302,8 +327,9 @@ struct TileLoad
     static_assert(kUnits % kWaveSize == 0, "whole waves");
     Eight<T> held[kDirect ? 1 : kEach];
 
-    __device__ __forceinline__ void issue(__amdgpu_buffer_rsrc_t b, int stride_bytes, int dim, LdsBytes tile, int t)
+    __device__ __forceinline__ void issue(const u32x4& buffer, int stride_bytes, int dim, LdsBytes tile, int t)
     {
+        const __amdgpu_buffer_rsrc_t b = resource_of(buffer);
 #pragma unroll
         for (int i = 0; i < kEach; ++i)
         {
@@ -313,9 +339,7 @@ struct TileLoad
             const int row = p / Tile<DP>::kChunks, at = 8 * Tile<DP>::chunk_at(row, p % Tile<DP>::kChunks);
             const unsigned int byte = row * stride_bytes + at * static_cast<int>(sizeof(T));
             if constexpr (kDirect)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                    b, reinterpret_cast<__attribute__((address_space(3))) void*>(tile + of_wave * 16), 16, at < dim ? byte : kOutside, 0,
-                    0, 0);
+                load_to_lds<16>(buffer, at < dim ? byte : kOutside, tile + of_wave * 16);
             else if constexpr (Whole)
             {
                 held[i].v[0] = __builtin_amdgcn_raw_buffer_load_b128(b, at < dim ? byte : kOutside, 0, 0);
@@ -362,12 +386,6 @@ struct TileLoad
     }
 };
 
-// 64 numbers of a buffer to LDS, by a wave.
-__device__ __forceinline__ void load_numbers(__amdgpu_buffer_rsrc_t b, LdsBytes to, int lane)
-{
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(b, reinterpret_cast<__attribute__((address_space(3))) void*>(to), 4, lane * 4, 0, 0, 0);
-}
-
 // ---- products --------------------------------------------------------------------------------------------------
 // A row's elements as second operand: what lane l has of row l % 32, for the contraction over DP elements.
 template <typename T, int DP>
@@ -409,6 +427,24 @@ __device__ __forceinline__ void multiply(const bf16x8 (&a)[3], const bf16x8 (&b)
     *s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], *s, 0, 0, 0);
 }
 
+// Order of Steps steps, each of Reads reads from LDS and Products products: reads run Ahead steps ahead.  (Left to itself the compiler reads
+// into the same registers at each step, and a wave waits for LDS before every product.)
+template <int Steps, int Reads, int Products, int Ahead = 6>
+__device__ __forceinline__ void read_ahead()
+{
+    constexpr int kAhead = Ahead < Steps ? Ahead : Steps, kRead = 0x100, kProduct = 0x8;
+    __builtin_amdgcn_sched_group_barrier(kRead, kAhead * Reads, 0);
+#pragma unroll
+    for (int i = 0; i < Steps - kAhead; ++i)
+    {
+        __builtin_amdgcn_sched_group_barrier(kProduct, Products, 0);
+        __builtin_amdgcn_sched_group_barrier(kRead, Reads, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(kProduct, kAhead * Products, 0);
+}
+template <typename T>
+constexpr int kProducts = kPlanes<T> == 1 ? 1 : 6; // of two elements
+
 // s[b] (m, n) = sum over DP of tile[first_row + 32 b + m] * row n of the fragment, of a tile of R rows: lane l's number i has n = l % 32 and
 // m = 8 (i / 4) + 4 (l / 32) + i % 4.  (The blocks' chains of products are interleaved: none waits for its own last one.)
 template <typename T, int DP, int R, int B>
@@ -433,6 +469,7 @@ __device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fra
                 a[p] = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(at + p * R * L::kRowBytes);
             multiply(a, f.chunk[c], &s[b]);
         }
+    read_ahead<DP / 16 * B, kPlanes<T>, kProducts<T>>();
 }
 template <typename T, int DP, int R>
 __device__ __forceinline__ f32x16 product(LdsBytes tile, int first_row, const Fragment<T, DP>& f)
@@ -466,6 +503,7 @@ __device__ __forceinline__ void two_products(LdsBytes tile_s, LdsBytes tile_t, i
         multiply(a, f.chunk[c], s);
         multiply(b, g.chunk[c], t);
     }
+    read_ahead<DP / 16, 2 * kPlanes<T>, 2 * kProducts<T>, 2>();
 }
 
 // 32 x 32 numbers as they come out of products(), as second operand of a contraction over m.
@@ -531,6 +569,7 @@ __device__ __forceinline__ void accumulate(LdsBytes tile, int first_row, const W
                 }
             multiply(a, b, &out[d]);
         }
+    read_ahead<DP / 16, 2 * kPlanes<T>, kProducts<T>>();
 }
 
 // Stores what accumulate() made of row l % 32 (v times factor), at p; Whole: rows begin on multiples of 16 bytes.

@@ -59,7 +59,7 @@ template <typename T, int DP, bool Whole>
 __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_dq_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
-    constexpr int KT = kTileRows<T>;
+    constexpr int KT = kTileRows<T>, B = KT / 32;
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, KT>];
     const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks);
     if (place.head >= a.heads)
@@ -144,24 +144,32 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
         if (tile + 1 < tiles)
             issue(tile + 1);
         const LdsBytes k_tile = (LdsBytes) lds[tile & 1][0], v_tile = (LdsBytes) lds[tile & 1][1];
-#pragma unroll
-        for (int b = 0; b < KT / 32; ++b)
+        const int at = from + tile * KT;
+        if (first <= last && at < some_end && at + KT > some_from)
         {
-            const int at = from + tile * KT + 32 * b;
-            if (first > last || at >= some_end || at + 32 <= some_from)
-                continue;
-            f32x16 s, dp;
-            two_products<T, DP, KT>(k_tile, v_tile, 32 * b, q, d_o, &s, &dp);
-            if (at < all_from || at + 32 > all_end)
-                hide(&s, at, row_from, row_end);
-            Weights<T> ds;
+            f32x16 s[B], dp[B];
+            products<T, DP, KT>(k_tile, 0, q, s);
+            products<T, DP, KT>(v_tile, 0, d_o, dp);
+            if (at < all_from || at + KT > all_end)
+            {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-                s[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[j], a.scale_log2, -log2_sum)) * (dp[j] - delta);
+                for (int b = 0; b < B; ++b)
+                    hide(&s[b], at + 32 * b, row_from, row_end);
+            }
+            Weights<T> ds[B];
 #pragma unroll
-            for (int j = 0; j < 16; j += 2)
-                ds.set(j, s[j], s[j + 1]);
-            accumulate<T, DP, KT>(k_tile, 32 * b, ds, dq);
+            for (int b = 0; b < B; ++b)
+            {
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    s[b][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j], a.scale_log2, -log2_sum)) * (dp[b][j] - delta);
+#pragma unroll
+                for (int j = 0; j < 16; j += 2)
+                    ds[b].set(j, s[b][j], s[b][j + 1]);
+            }
+#pragma unroll
+            for (int b = 0; b < B; ++b)
+                accumulate<T, DP, KT>(k_tile, 32 * b, ds[b], dq);
         }
         if (tile + 1 < tiles)
             put(tile + 1); // (all waves are past the tile that lay there)
@@ -180,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
 {
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr bool kOneWave = DP == 128 || kWavesOf<T, DP, Whole> == 1; // (128 elements: two waves would have to spill)
-    constexpr int QT = kTileRows<T>;
+    constexpr int QT = kTileRows<T>, B = QT / 32;
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, QT>];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kWaveSize];
     const int key_heads = a.query_heads / a.group;
@@ -214,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
         {
             const float* const p = (wave == 0 ? a.log2_sum : a.delta)
                                    + (static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + at;
-            load_numbers(buffer_of(p, rows, 1, 1), (LdsBytes) stats[stage][wave], lane);
+            load_to_lds<4>(buffer_of(p, rows, 1, 1), 4 * lane, (LdsBytes) stats[stage][wave]);
         }
     };
     const auto put = [&](int stage) {
@@ -251,41 +259,45 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
         if (step + 1 < steps)
             issue(g, tile, stage ^ 1);
         const LdsBytes q_tile = (LdsBytes) lds[stage][0], d_o_tile = (LdsBytes) lds[stage][1];
-#pragma unroll
-        for (int b = 0; b < QT / 32; ++b)
+        const float* const log2_sum = &stats[stage][0][4 * (lane / 32)];
+        const float* const delta = &stats[stage][1][4 * (lane / 32)];
+        if (first <= last && here < some_end && here + QT > some_from)
         {
-            const int at = here + 32 * b;
-            if (first > last || at >= some_end || at + 32 <= some_from)
-                continue;
-            const float* const log2_sum = &stats[stage][0][32 * b + 4 * (lane / 32)];
-            const float* const delta = &stats[stage][1][32 * b + 4 * (lane / 32)];
-            Weights<T> p, ds;
-            f32x16 s = product<T, DP, QT>(q_tile, 32 * b, k);
-            if (at < all_from || at + 32 > all_end)
-                hide(&s, at, row_from, row_end);
-#pragma unroll
-            for (int r = 0; r < 16; r += 4)
+            // All blocks of the tile in one go: the products of one run beside the exponentials of another.
+            f32x16 s[B], dp[B];
+            products<T, DP, QT>(q_tile, 0, k, s);
+            products<T, DP, QT>(d_o_tile, 0, v, dp);
+            if (here < all_from || here + QT > all_end)
             {
-                const f32x4 l = *reinterpret_cast<const f32x4*>(log2_sum + 2 * r);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    s[r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r + e], a.scale_log2, -l[e]));
-                p.set(r, s[r], s[r + 1]);
-                p.set(r + 2, s[r + 2], s[r + 3]);
+                for (int b = 0; b < B; ++b)
+                    hide(&s[b], here + 32 * b, row_from, row_end);
             }
-            accumulate<T, DP, QT>(d_o_tile, 32 * b, p, dv);
-            const f32x16 dp = product<T, DP, QT>(d_o_tile, 32 * b, v);
+            Weights<T> p[B], ds[B];
 #pragma unroll
-            for (int r = 0; r < 16; r += 4)
+            for (int b = 0; b < B; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; r += 4)
+                {
+                    const f32x4 l = *reinterpret_cast<const f32x4*>(log2_sum + 32 * b + 2 * r);
+                    const f32x4 m = *reinterpret_cast<const f32x4*>(delta + 32 * b + 2 * r);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                    {
+                        s[b][r + e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][r + e], a.scale_log2, -l[e]));
+                        dp[b][r + e] = s[b][r + e] * (dp[b][r + e] - m[e]);
+                    }
+                    p[b].set(r, s[b][r], s[b][r + 1]);
+                    p[b].set(r + 2, s[b][r + 2], s[b][r + 3]);
+                    ds[b].set(r, dp[b][r], dp[b][r + 1]);
+                    ds[b].set(r + 2, dp[b][r + 2], dp[b][r + 3]);
+                }
+#pragma unroll
+            for (int b = 0; b < B; ++b)
             {
-                const f32x4 l = *reinterpret_cast<const f32x4*>(delta + 2 * r);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    s[r + e] *= dp[r + e] - l[e];
-                ds.set(r, s[r], s[r + 1]);
-                ds.set(r + 2, s[r + 2], s[r + 3]);
+                accumulate<T, DP, QT>(d_o_tile, 32 * b, p[b], dv);
+                accumulate<T, DP, QT>(q_tile, 32 * b, ds[b], dk);
             }
-            accumulate<T, DP, QT>(q_tile, 32 * b, ds, dk);
         }
         if (step + 1 < steps)
             put(stage ^ 1);
