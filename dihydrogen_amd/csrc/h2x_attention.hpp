@@ -387,20 +387,21 @@ struct TileLoad
 };
 
 // ---- products --------------------------------------------------------------------------------------------------
-// A row's elements as second operand: what lane l has of row l % 32, for the contraction over DP elements.
-template <typename T, int DP>
+// A row's elements as second operand: what lane l has of row l % 32, for the contraction over DQ elements (a multiple of 16; tiles in LDS have a
+// multiple of 32, DP).
+template <typename T, int DQ>
 struct Fragment
 {
-    bf16x8 chunk[DP / 16][kPlanes<T>]; // elements 16 c + 8 (lane / 32) and on
+    bf16x8 chunk[DQ / 16][kPlanes<T>]; // elements 16 c + 8 (lane / 32) and on
 };
 
 // Of the row at p; zero where it is not `there`.
-template <typename T, int DP, bool Whole>
-__device__ __forceinline__ void load_fragment(Fragment<T, DP>* f, const T* p, bool there, int dim)
+template <typename T, int DQ, bool Whole>
+__device__ __forceinline__ void load_fragment(Fragment<T, DQ>* f, const T* p, bool there, int dim)
 {
     const int half = (threadIdx.x & (kWaveSize - 1)) / 32;
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
+    for (int c = 0; c < DQ / 16; ++c)
         planes_of(load_eight<T, Whole>(p, 16 * c + 8 * half, there, dim), f->chunk[c]);
 }
 
@@ -445,10 +446,10 @@ __device__ __forceinline__ void read_ahead()
 template <typename T>
 constexpr int kProducts = kPlanes<T> == 1 ? 1 : 6; // of two elements
 
-// s[b] (m, n) = sum over DP of tile[first_row + 32 b + m] * row n of the fragment, of a tile of R rows: lane l's number i has n = l % 32 and
+// s[b] (m, n) = sum over DQ of tile[first_row + 32 b + m] * row n of the fragment, of a tile of R rows: lane l's number i has n = l % 32 and
 // m = 8 (i / 4) + 4 (l / 32) + i % 4.  (The blocks' chains of products are interleaved: none waits for its own last one.)
-template <typename T, int DP, int R, int B>
-__device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fragment<T, DP>& f, f32x16 (&s)[B])
+template <typename T, int DP, int DQ, int R, int B>
+__device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fragment<T, DQ>& f, f32x16 (&s)[B])
 {
     using L = Tile<DP>;
     const int lane = threadIdx.x & (kWaveSize - 1);
@@ -457,7 +458,7 @@ __device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fra
     for (int b = 0; b < B; ++b)
         s[b] = zero16();
 #pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
+    for (int c = 0; c < DQ / 16; ++c)
 #pragma unroll
         for (int b = 0; b < B; ++b)
         {
@@ -469,43 +470,8 @@ __device__ __forceinline__ void products(LdsBytes tile, int first_row, const Fra
                 a[p] = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(at + p * R * L::kRowBytes);
             multiply(a, f.chunk[c], &s[b]);
         }
-    read_ahead<DP / 16 * B, kPlanes<T>, kProducts<T>>();
+    read_ahead<DQ / 16 * B, kPlanes<T>, kProducts<T>>();
 }
-template <typename T, int DP, int R>
-__device__ __forceinline__ f32x16 product(LdsBytes tile, int first_row, const Fragment<T, DP>& f)
-{
-    f32x16 s[1];
-    products<T, DP, R>(tile, first_row, f, s);
-    return s[0];
-}
-
-// The same of two tiles' rows with a fragment each, 32 rows: s from the first, t from the second.
-template <typename T, int DP, int R>
-__device__ __forceinline__ void two_products(LdsBytes tile_s, LdsBytes tile_t, int first_row, const Fragment<T, DP>& f,
-                                             const Fragment<T, DP>& g, f32x16* s, f32x16* t)
-{
-    using L = Tile<DP>;
-    const int lane = threadIdx.x & (kWaveSize - 1);
-    const int base = L::address(lane & 31, lane / 32);
-    *s = zero16();
-    *t = zero16();
-#pragma unroll
-    for (int c = 0; c < DP / 16; ++c)
-    {
-        const int at = first_row * L::kRowBytes + (L::kFlips ? base ^ 32 * c : L::address(lane & 31, 2 * c + lane / 32));
-        bf16x8 a[kPlanes<T>], b[kPlanes<T>];
-#pragma unroll
-        for (int p = 0; p < kPlanes<T>; ++p)
-        {
-            a[p] = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(tile_s + at + p * R * L::kRowBytes);
-            b[p] = *reinterpret_cast<__attribute__((address_space(3))) bf16x8*>(tile_t + at + p * R * L::kRowBytes);
-        }
-        multiply(a, f.chunk[c], s);
-        multiply(b, g.chunk[c], t);
-    }
-    read_ahead<DP / 16, 2 * kPlanes<T>, 2 * kProducts<T>, 2>();
-}
-
 // 32 x 32 numbers as they come out of products(), as second operand of a contraction over m.
 template <typename T>
 struct Weights
@@ -685,14 +651,21 @@ inline Schedule schedule_of(const h2x_attention& a, bool keys, uint64_t heads, u
     return {right != keys ? kLastFirst : kFirstFirst, static_cast<int>(blocks)};
 }
 
-// f(std::integral_constant<int, DP>) for heads padded to a multiple of 32 elements.
+// Elements of a head in LDS, a multiple of 32, and in a contraction, of 16.
+template <int P, int Q>
+struct Padded
+{
+    static constexpr int in_lds = P, contracted = Q;
+};
+// f(Padded()) for heads of `dim` elements.
 template <typename F>
 int with_padded_dim(int dim, const F& f)
 {
-    return dim <= 32   ? f(std::integral_constant<int, 32>())
-           : dim <= 64 ? f(std::integral_constant<int, 64>())
-           : dim <= 96 ? f(std::integral_constant<int, 96>())
-                       : f(std::integral_constant<int, 128>());
+    return dim <= 32   ? f(Padded<32, 32>())
+           : dim <= 64 ? f(Padded<64, 64>())
+           : dim <= 80 ? f(Padded<96, 80>()) // (72 and 80 are common; a sixth of two products)
+           : dim <= 96 ? f(Padded<96, 96>())
+                       : f(Padded<128, 128>());
 }
 
 // f(T(), Whole) for the type of the elements.

@@ -55,7 +55,7 @@ struct Args
 };
 
 // dq, and what the other pass needs of each row.  As in the forward pass, the waves of a workgroup take 32 queries of a head each.
-template <typename T, int DP, bool Whole>
+template <typename T, int DP, int DQ, bool Whole>
 __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_dq_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -100,13 +100,13 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
 
     const bool there = i <= last;
     const int64_t row = (static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + i;
-    Fragment<T, DP> q, d_o;
+    Fragment<T, DQ> q, d_o;
     float delta = 0.0f, log2_sum = -kLowest;
     {
         const T* const o_row = a.o + n * a.os.sample + head * a.os.head + i * a.os.token;
         const T* const d_o_row = a.d_o + n * a.d_os.sample + head * a.d_os.head + i * a.d_os.token;
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c)
+        for (int c = 0; c < DQ / 16; ++c)
         {
             const int at = 16 * c + 8 * (lane / 32);
             const Eight<T> x = load_eight<T, Whole>(o_row, at, there, a.dim), y = load_eight<T, Whole>(d_o_row, at, there, a.dim);
@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
         }
         delta = halves_sum(delta);
     }
-    load_fragment<T, DP, Whole>(&q, a.q + n * a.qs.sample + head * a.qs.head + i * a.qs.token, there, a.dim);
+    load_fragment<T, DQ, Whole>(&q, a.q + n * a.qs.sample + head * a.qs.head + i * a.qs.token, there, a.dim);
     if (there)
     {
         const float l = a.logsumexp[row];
@@ -148,8 +148,8 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
         if (first <= last && at < some_end && at + KT > some_from)
         {
             f32x16 s[B], dp[B];
-            products<T, DP, KT>(k_tile, 0, q, s);
-            products<T, DP, KT>(v_tile, 0, d_o, dp);
+            products<T, DP, DQ, KT>(k_tile, 0, q, s);
+            products<T, DP, DQ, KT>(v_tile, 0, d_o, dp);
             if (at < all_from || at + KT > all_end)
             {
 #pragma unroll
@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
 
 // dk and dv: the waves of a workgroup take 32 keys of a key head each; the queries of the heads that share it pass through LDS, one head after
 // another.
-template <typename T, int DP, bool Whole>
+template <typename T, int DP, int DQ, bool Whole>
 __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Whole>)) attention_dkv_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -237,9 +237,9 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
     }
 
     const bool there = j <= last;
-    Fragment<T, DP> k, v;
-    load_fragment<T, DP, Whole>(&k, a.k + n * a.ks.sample + key_head * a.ks.head + j * a.ks.token, there, a.dim);
-    load_fragment<T, DP, Whole>(&v, a.v + n * a.vs.sample + key_head * a.vs.head + j * a.vs.token, there, a.dim);
+    Fragment<T, DQ> k, v;
+    load_fragment<T, DQ, Whole>(&k, a.k + n * a.ks.sample + key_head * a.ks.head + j * a.ks.token, there, a.dim);
+    load_fragment<T, DQ, Whole>(&v, a.v + n * a.vs.sample + key_head * a.vs.head + j * a.vs.token, there, a.dim);
     f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -265,8 +265,8 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
         {
             // All blocks of the tile in one go: the products of one run beside the exponentials of another.
             f32x16 s[B], dp[B];
-            products<T, DP, QT>(q_tile, 0, k, s);
-            products<T, DP, QT>(d_o_tile, 0, v, dp);
+            products<T, DP, DQ, QT>(q_tile, 0, k, s);
+            products<T, DP, DQ, QT>(d_o_tile, 0, v, dp);
             if (here < all_from || here + QT > all_end)
             {
 #pragma unroll
@@ -335,20 +335,20 @@ int issue(const h2x_attention& c, Args<T> a, hipStream_t stream)
         return H2X_ERR_TOO_LARGE;
     const auto grid = [](uint64_t groups) { return dim3(static_cast<uint32_t>((groups + kNumXcd - 1) / kNumXcd * kNumXcd)); };
     return with_padded_dim(c.head_dim, [&](auto dim) {
-        constexpr int DP = decltype(dim)::value;
+        constexpr int DP = decltype(dim)::in_lds, DQ = decltype(dim)::contracted;
         if (query_groups > 0)
         {
             a.blocks = static_cast<int>(query_blocks);
             a.heads = c.samples * c.query_heads;
             a.schedule = schedule_of(c, false, a.heads, query_blocks);
-            launch(attention_dq_kernel<T, DP, Whole>, grid(query_groups), dim3(kThreads), stream, a);
+            launch(attention_dq_kernel<T, DP, DQ, Whole>, grid(query_groups), dim3(kThreads), stream, a);
         }
         if (key_groups > 0)
         {
             a.blocks = static_cast<int>(key_blocks);
             a.heads = c.samples * c.key_heads;
             a.schedule = schedule_of(c, true, a.heads, key_blocks);
-            launch(attention_dkv_kernel<T, DP, Whole>, grid(key_groups), dim3(kThreads), stream, a);
+            launch(attention_dkv_kernel<T, DP, DQ, Whole>, grid(key_groups), dim3(kThreads), stream, a);
         }
         return launch_status();
     });

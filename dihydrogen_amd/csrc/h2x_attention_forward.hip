@@ -39,10 +39,10 @@ struct Args
 };
 
 // A wave's 32 rows.
-template <typename T, int DP>
+template <typename T, int DP, int DQ>
 struct Rows32
 {
-    Fragment<T, DP> q;
+    Fragment<T, DQ> q;
     f32x16 out[DP / 32]; // unnormalised
     float max, sum;      // the maximum in units of log2; the sum over this half's keys
     int from, end;       // keys that the lane's row sees
@@ -59,7 +59,7 @@ struct Rows32
     // The scores of a tile's keys.
     __device__ __forceinline__ void score(LdsBytes k_tile, f32x16 (&s)[kTileKeys<T> / 32]) const
     {
-        products<T, DP, kTileKeys<T>>(k_tile, 0, q, s);
+        products<T, DP, DQ, kTileKeys<T>>(k_tile, 0, q, s);
     }
 
     // Scores to probabilities, with maximum, sum and output brought up to date.
@@ -118,7 +118,7 @@ struct Rows32
 
 // Many queries: the waves of a workgroup take 32 queries of a head each, and share the tiles of keys and values, which come
 // straight from memory to LDS while the tile before them is worked on.
-template <typename T, int DP, bool Whole>
+template <typename T, int DP, int DQ, bool Whole>
 __global__ void __launch_bounds__(kThreads, (sizeof(T) == 2 || DP <= 96 ? 2 : 1)) attention_forward_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -162,9 +162,9 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 2 || DP <= 96 ? 2 : 1)
         put(0);
     }
 
-    Rows32<T, DP> rows;
+    Rows32<T, DP, DQ> rows;
     rows.clear();
-    load_fragment<T, DP, Whole>(&rows.q, a.q + n * a.qs.sample + head * a.qs.head + i * a.qs.token, i <= last, a.dim);
+    load_fragment<T, DQ, Whole>(&rows.q, a.q + n * a.qs.sample + head * a.qs.head + i * a.qs.token, i <= last, a.dim);
     rows.from = sample.first_key(min(i, max(last, 0)));
     rows.end = sample.end_key(min(i, max(last, 0)));
     // keys that some, and that all rows of the wave see
@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 2 || DP <= 96 ? 2 : 1)
 // Few workgroups' worth of queries: the queries of all heads that share a key head are rows one after another, 32 of them a workgroup, so
 // that keys and values are read once for them.  The waves of a workgroup go through different tiles of the same part of the keys,
 // each with LDS of its own and without barriers, and join what they have at the end.
-template <typename T, int DP, bool Whole>
+template <typename T, int DP, int DQ, bool Whole>
 __global__ void __launch_bounds__(kThreads) attention_split_kernel(const Args<T> a)
 {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -251,10 +251,10 @@ __global__ void __launch_bounds__(kThreads) attention_split_kernel(const Args<T>
                     a.dim, to, lane);
     };
 
-    Rows32<T, DP> rows;
+    Rows32<T, DP, DQ> rows;
     rows.clear();
     const bool there = i <= last_query;
-    load_fragment<T, DP, Whole>(&rows.q, a.q + n * a.qs.sample + head * a.qs.head + i * a.qs.token, there, a.dim);
+    load_fragment<T, DQ, Whole>(&rows.q, a.q + n * a.qs.sample + head * a.qs.head + i * a.qs.token, there, a.dim);
     rows.from = there ? sample.first_key(i) : 0;
     rows.end = there ? sample.end_key(i) : 0;
     const int all_from = sample.first_key(last_query), all_end = sample.end_key(first_query);
@@ -478,11 +478,11 @@ int issue(const h2x_attention& c, const Plan& p, const Args<T>& a, hipStream_t s
 {
     const dim3 grid(static_cast<uint32_t>((p.groups + kNumXcd - 1) / kNumXcd * kNumXcd));
     return with_padded_dim(c.head_dim, [&](auto dim) {
-        constexpr int DP = decltype(dim)::value;
+        constexpr int DP = decltype(dim)::in_lds, DQ = decltype(dim)::contracted;
         if (p.split)
-            launch(attention_split_kernel<T, DP, Whole>, grid, dim3(kThreads), stream, a);
+            launch(attention_split_kernel<T, DP, DQ, Whole>, grid, dim3(kThreads), stream, a);
         else
-            launch(attention_forward_kernel<T, DP, Whole>, grid, dim3(kThreads), stream, a);
+            launch(attention_forward_kernel<T, DP, DQ, Whole>, grid, dim3(kThreads), stream, a);
         if (p.parts > 4)
             launch(attention_join_kernel<T, DP, 4>, dim3(static_cast<uint32_t>(rows_of(c))), dim3(kThreads), stream, a);
         else if (p.parts > 1)
