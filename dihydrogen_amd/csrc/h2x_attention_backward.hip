@@ -71,18 +71,20 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
     const int block_first = block * (kWaves * kRows), block_end = min(block_first + kWaves * kRows, sample.queries);
     const int first = block_first + wave * kRows, i = first + (lane & 31);
     const int last = min(first + kRows, sample.queries) - 1;
-    int from = 0, tiles = 0;
+    // keys that some row of the workgroup sees; what else lies in their tiles is read as zero
+    int from = 0, to = 0;
     if (block_first < block_end)
     {
         from = sample.first_key(block_first);
-        tiles = (max(sample.end_key(block_end - 1) - from, 0) + KT - 1) / KT;
+        to = sample.end_key(block_end - 1);
     }
+    const int tiles = (max(to - from, 0) + KT - 1) / KT;
     const T* const k = a.k + n * a.ks.sample + (head / a.group) * a.ks.head;
     const T* const v = a.v + n * a.vs.sample + (head / a.group) * a.vs.head;
     const int k_bytes = static_cast<int>(a.ks.token * sizeof(T)), v_bytes = static_cast<int>(a.vs.token * sizeof(T));
     TileLoad<T, DP, KT, kThreads, Whole> k_load, v_load;
     const auto issue = [&](int tile) {
-        const int at = from + tile * KT, rows = min(KT, sample.keys - at);
+        const int at = from + tile * KT, rows = min(KT, to - at);
         k_load.issue(buffer_of(k + at * a.ks.token, rows, a.ks.token, a.dim), k_bytes, a.dim, (LdsBytes) lds[tile & 1][0],
                      threadIdx.x);
         v_load.issue(buffer_of(v + at * a.vs.token, rows, a.vs.token, a.dim), v_bytes, a.dim, (LdsBytes) lds[tile & 1][1],
@@ -98,7 +100,8 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
         put(0);
     }
 
-    const bool there = i <= last;
+    const int row_from = sample.first_key(min(i, max(last, 0))), row_end = sample.end_key(min(i, max(last, 0)));
+    const bool there = i <= last && row_from < row_end; // (a row that sees no key may hold anything)
     const int64_t row = (static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + i;
     Fragment<T, DQ> q, d_o;
     float delta = 0.0f, log2_sum = -kLowest;
@@ -133,7 +136,6 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
         dq[d] = zero16();
-    const int row_from = sample.first_key(min(i, max(last, 0))), row_end = sample.end_key(min(i, max(last, 0)));
     const int some_from = sample.first_key(first), some_end = sample.end_key(last);
     const int all_from = sample.first_key(last), all_end = sample.end_key(first);
 
@@ -202,17 +204,18 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
     const int block_first = block * (kWaves * kRows), block_end = min(block_first + kWaves * kRows, sample.keys);
     const int first = block_first + wave * kRows, j = first + (lane & 31);
     const int last = min(first + kRows, sample.keys) - 1;
-    int from = 0, tiles = 0;
+    int from = 0, to = 0;
     if (block_first < block_end)
     {
         from = sample.first_query(block_first);
-        tiles = (max(sample.end_query(block_end - 1) - from, 0) + QT - 1) / QT;
+        to = sample.end_query(block_end - 1);
     }
+    const int tiles = (max(to - from, 0) + QT - 1) / QT;
     const int q_bytes = static_cast<int>(a.qs.token * sizeof(T)), d_o_bytes = static_cast<int>(a.d_os.token * sizeof(T));
     TileLoad<T, DP, QT, kThreads, Whole> q_load, d_o_load;
     // tile `tile` of the group's head `g`, to stage `stage`
     const auto issue = [&](int g, int tile, int stage) {
-        const int head = key_head * a.group + g, at = from + tile * QT, rows = min(QT, sample.queries - at);
+        const int head = key_head * a.group + g, at = from + tile * QT, rows = min(QT, to - at);
         const T* const q = a.q + n * a.qs.sample + head * a.qs.head + at * a.qs.token;
         const T* const d_o = a.d_o + n * a.d_os.sample + head * a.d_os.head + at * a.d_os.token;
         q_load.issue(buffer_of(q, rows, a.qs.token, a.dim), q_bytes, a.dim, (LdsBytes) lds[stage][0], threadIdx.x);
@@ -236,7 +239,8 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
         put(0);
     }
 
-    const bool there = j <= last;
+    const int row_from = sample.first_query(min(j, max(last, 0))), row_end = sample.end_query(min(j, max(last, 0)));
+    const bool there = j <= last && row_from < row_end; // (a key that no query sees may hold anything)
     Fragment<T, DQ> k, v;
     load_fragment<T, DQ, Whole>(&k, a.k + n * a.ks.sample + key_head * a.ks.head + j * a.ks.token, there, a.dim);
     load_fragment<T, DQ, Whole>(&v, a.v + n * a.vs.sample + key_head * a.vs.head + j * a.vs.token, there, a.dim);
@@ -244,7 +248,6 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
         dk[d] = dv[d] = zero16();
-    const int row_from = sample.first_query(min(j, max(last, 0))), row_end = sample.end_query(min(j, max(last, 0)));
     const int some_from = sample.first_query(first), some_end = sample.end_query(last);
     const int all_from = sample.first_query(last), all_end = sample.end_query(first);
 

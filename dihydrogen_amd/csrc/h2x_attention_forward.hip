@@ -135,18 +135,20 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 2 || DP <= 96 ? 2 : 1)
     const int block_first = block * (kWaves * kRows), block_end = min(block_first + kWaves * kRows, sample.queries);
     const int first = block_first + wave * kRows, i = first + (lane & 31);
     const int last = min(first + kRows, sample.queries) - 1; // (of the wave; before first: it has none)
-    int from = 0, tiles = 0;
+    // keys that some row of the workgroup sees; what else lies in their tiles is read as zero
+    int from = 0, to = 0;
     if (block_first < block_end)
     {
         from = sample.first_key(block_first);
-        tiles = (max(sample.end_key(block_end - 1) - from, 0) + KT - 1) / KT;
+        to = sample.end_key(block_end - 1);
     }
+    const int tiles = (max(to - from, 0) + KT - 1) / KT;
     const T* const k = a.k + n * a.ks.sample + (head / a.group) * a.ks.head;
     const T* const v = a.v + n * a.vs.sample + (head / a.group) * a.vs.head;
     const int k_bytes = static_cast<int>(a.ks.token * sizeof(T)), v_bytes = static_cast<int>(a.vs.token * sizeof(T));
     TileLoad<T, DP, KT, kThreads, Whole> k_load, v_load;
     const auto issue = [&](int tile) {
-        const int at = from + tile * KT, rows = min(KT, sample.keys - at);
+        const int at = from + tile * KT, rows = min(KT, to - at);
         k_load.issue(buffer_of(k + at * a.ks.token, rows, a.ks.token, a.dim), k_bytes, a.dim, (LdsBytes) lds[tile & 1][0],
                      threadIdx.x);
         v_load.issue(buffer_of(v + at * a.vs.token, rows, a.vs.token, a.dim), v_bytes, a.dim, (LdsBytes) lds[tile & 1][1],
@@ -232,12 +234,13 @@ __global__ void __launch_bounds__(kThreads) attention_split_kernel(const Args<T>
     const bool one_head = first / queries == last / queries;
     const int first_query = one_head ? first - first / queries * queries : 0;
     const int last_query = min(one_head ? last - last / queries * queries : queries - 1, sample.queries - 1);
-    int from = 0, tiles = 0;
+    int from = 0, to = 0;
     if (first_query <= last_query)
     {
         from = sample.first_key(first_query);
-        tiles = (max(sample.end_key(last_query) - from, 0) + KT - 1) / KT;
+        to = sample.end_key(last_query);
     }
+    const int tiles = (max(to - from, 0) + KT - 1) / KT;
     const int first_tile = static_cast<int>(static_cast<int64_t>(tiles) * part / a.parts.num);
     const int end_tile = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / a.parts.num);
 
@@ -245,10 +248,10 @@ __global__ void __launch_bounds__(kThreads) attention_split_kernel(const Args<T>
     const T* const v = a.v + n * a.vs.sample + key_head * a.vs.head;
     const LdsBytes k_tile = (LdsBytes) (lds + wave * (Load::kDirect ? 2 : 1) * kBytes), v_tile = k_tile + (Load::kDirect ? kBytes : 0);
     Load k_load, v_load;
-    const auto issue = [&](Load* load, const T* p, const Strides& s, int tile, LdsBytes to) {
+    const auto issue = [&](Load* load, const T* p, const Strides& s, int tile, LdsBytes lds_tile) {
         const int at = from + tile * KT;
-        load->issue(buffer_of(p + at * s.token, min(KT, sample.keys - at), s.token, a.dim), static_cast<int>(s.token * sizeof(T)),
-                    a.dim, to, lane);
+        load->issue(buffer_of(p + at * s.token, min(KT, to - at), s.token, a.dim), static_cast<int>(s.token * sizeof(T)),
+                    a.dim, lds_tile, lane);
     };
 
     Rows32<T, DP, DQ> rows;

@@ -549,6 +549,8 @@ __global__ void __launch_bounds__(kSumColumns* kSumLanes)
 
 // ---- host ----------------------------------------------------------------------
 
+constexpr int kMostChannels = 1 << 26; // a grid of fewer than 2^32 threads for the weights' sums
+
 // How the rows are shared out: the fewest threads whose registers hold a row, at 128 bytes of sums' type a thread, or 96 where a
 // workgroup of 512 threads leaves each 256 registers (the backward pass keeps four numbers an element).
 struct Split
@@ -696,7 +698,7 @@ extern "C" int h2x_layer_norm_forward(h2x_dtype dtype, h2x_dtype weight_dtype, s
         using P = decltype(p);
         if (num_channels < 1 || !(epsilon >= 0) || (mean == nullptr) != (rstd == nullptr))
             return H2X_ERR_INVALID_ARGUMENT;
-        if (num_rows > 0x7fffffffu)
+        if (num_rows > 0x7fffffffu || num_channels > kMostChannels)
             return H2X_ERR_TOO_LARGE;
         Forward<T, P> a{static_cast<const T*>(x), static_cast<const P*>(scale), static_cast<const P*>(bias),
                         static_cast<T*>(y),       static_cast<wide<T>*>(mean),  static_cast<wide<T>*>(rstd)};
@@ -733,7 +735,7 @@ extern "C" int h2x_layer_norm_backward(h2x_dtype dtype, h2x_dtype weight_dtype, 
         using P = decltype(p);
         if (num_channels < 1)
             return H2X_ERR_INVALID_ARGUMENT;
-        if (num_rows > 0x7fffffffu)
+        if (num_rows > 0x7fffffffu || num_channels > kMostChannels)
             return H2X_ERR_TOO_LARGE;
         const bool weights = dscale || dbias;
         Backward<T, P> a{static_cast<const T*>(x),          static_cast<const T*>(dy),

@@ -3,6 +3,7 @@
 //   distconv::tensor::HaloExchange / HaloExchangeVirtual,
 //   distconv::tensor::TensorMPICUDAShuffler / TensorShufflerVirtual,
 //   distconv::tensor::Transform / ReduceSum / TransformReduceSum,
+//   distconv::LayerNormalization / RotaryPositions / Attention<BackendMI355X>,
 // and the tensor model they are written against.  Link with libh2x.so.
 #pragma once
 
@@ -11,6 +12,7 @@
 #include "distconv/halo_shuffle_mi355x.hpp"
 #include "distconv/layers_mi355x.hpp"
 #include "distconv/tensor_mi355x.hpp"
+#include "distconv/tokens_mi355x.hpp"
 
 #include <fstream>
 #include <string>

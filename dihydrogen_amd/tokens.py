@@ -89,6 +89,10 @@ def _rows(t: torch.Tensor) -> Optional[capi.TensorGeometry]:
     return g
 
 
+def _require_own_memory(*outputs: torch.Tensor) -> None:
+    _require(all(n <= 1 or s != 0 for t in outputs for n, s in zip(t.shape, t.stride())), "the elements of an output lie apart")
+
+
 def _address(struct) -> Optional[int]:
     return None if struct is None else ctypes.addressof(struct)
 
@@ -127,6 +131,7 @@ class LayerNormalization:
         for s in saved:
             _require(s is None or (s.dtype == kept and s.numel() == rows and s.is_contiguous()),
                      f"mean and rstd: one contiguous {kept} a row")
+        _require_own_memory(others[-1])
         geometries = [_rows(t) for t in (x, *others)]
         _on_one_gpu(device, self.stream, x, *others, *weights, *saved)
         return self._plans.keep(key, (dtype, _DTYPES[weight_dtype], rows, channels, [_address(g) for g in geometries], geometries))
@@ -223,6 +228,7 @@ class RotaryPositions:
         _require(x.dtype in _DTYPES, f"rotary positions of {x.dtype} elements are not supported")
         _require(_is_token_tensor(x) and _is_token_tensor(y), "(samples, tokens, heads, elements), the elements contiguous")
         _require(x.shape == y.shape and x.dtype == y.dtype, "tensors of one shape and type")
+        _require_own_memory(y)
         n, tokens, heads, dim = x.shape
         _require(dim == self.head_dim, f"heads of {self.head_dim} elements, not {dim}")
         axes = len(self.axis_pairs)
@@ -270,7 +276,7 @@ class Attention:
     own place to `right` behind it; None: no bound.  ``causal``: no key behind its own place.
     ``query_lengths``, ``key_lengths``: int32 on the GPU, one a sample, for padded batches and caches; None: samples are whole.  Rows behind a
     sample's lengths are not read; their outputs and gradients are zero, as are those of queries that see no key, whose logsumexp is minus infinity.
-    Keys and values within the lengths have to be finite.
+    Keys and values that any query sees have to be finite (float32: below 3e38).
     """
 
     def __init__(self, scale: Optional[float] = None, causal: bool = False,
@@ -299,6 +305,7 @@ class Attention:
         _require(q.dtype in (torch.bfloat16, torch.float32), f"attention of {q.dtype} elements is not supported")
         _require(all(_is_token_tensor(t) and t.dtype == q.dtype for t in tensors),
                  "(samples, tokens, heads, elements) of one type, the elements contiguous")
+        _require_own_memory(*(gradients[1:] or (o,)))
         n, queries, heads, dim = q.shape
         keys, key_heads = k.shape[1:3]
         like_q, like_k = (o, *gradients[:2]), (v, *gradients[2:])

@@ -1330,7 +1330,7 @@ int h2x_shuffle_direct(const h2x_shuffle_direct_plan* plan, void* const* src, vo
  * of 1 to H2X_MAX_DIMS dimensions with local_shape[0] == num_channels, strides[0] == 1 and num_rows as
  * the product of the other extents, r counting through them innermost first (the interior of a
  * haloed tensor whose channel is innermost).  y may be x itself, with the same rows.  Sums are in 32 bits (64
- * with H2X_F64), the squares' about the mean.  num_rows up to 2^31 - 1.
+ * with H2X_F64), the squares' about the mean.  num_rows up to 2^31 - 1, num_channels up to 2^26.
  */
 int h2x_layer_norm_forward(h2x_dtype dtype,
                            h2x_dtype weight_dtype,
@@ -1402,8 +1402,8 @@ typedef struct h2x_rotary
 {
     int32_t dtype; /* any h2x_dtype */
     int32_t pairing;
-    int32_t head_dim, heads, samples, num_axes;
-    int64_t tokens;
+    int32_t head_dim, heads, samples, num_axes; /* head_dim: 1 to 256 */
+    int64_t tokens; /* below 2^31 */
     int32_t axis_pairs[H2X_MAX_AXES];
     /* element (sample, axis, token) of positions lies at sample * positions_sample_stride + axis * positions_axis_stride +
      * token; a sample stride of 0: all samples have the same */
@@ -1432,7 +1432,8 @@ int h2x_rotary_apply(const h2x_rotary* rotary,
  * values are clamped to 0 and these).  What lies behind a sample's lengths is not used, whatever its values.
  * Mask: the last query of a sample stands at its last key, so query i stands at place(i) = i + its keys - its queries, and sees the keys
  * j with place(i) - window_left <= j <= place(i) + window_right; a negative window_left or window_right has no bound
- * (window_right = 0: a query sees no key behind its own place).  Keys and values within a sample's lengths have to be finite.
+ * (window_right = 0: a query sees no key behind its own place).  Keys and values that any query sees have to be finite (floats: below 3e38);
+ * what no query sees may hold anything.
  * Empty rows (a query that sees no key, or lies behind its sample's queries) have output zero and a logarithm of minus infinity, and give
  * no gradients; rows of the gradients behind the lengths are zero.
  */

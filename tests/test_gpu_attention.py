@@ -158,6 +158,36 @@ def test_rising_scores(dtype):
         p.check()
 
 
+@DTYPES
+def test_what_no_query_sees_may_hold_anything(dtype):
+    """Keys before a window's reach and behind the last query's, a tile or a few keys of them, within the sample's lengths."""
+    for queries, window in ((1, (20, 0)), (3, (70, 0)), (40, (10, 0)), (130, (100, 0)), (1, (0, 0))):
+        p = Problem(2, queries, 300, 4, 2, 64, dtype, window=window)
+        q, k, v, _ = p.inputs
+        unseen = ~p.seen.any(1)[0].cuda()
+        assert bool(unseen.any())
+        clean = [t.clone() for t in (k, v)]
+        for t in (k, v):
+            t[:, unseen] = torch.tensor([math.nan, math.inf, -math.inf, 1e30], device="cuda").repeat(128)[:int(unseen.sum())].to(dtype)[:, None, None]
+        p.check()
+        k.copy_(clean[0]), v.copy_(clean[1])
+
+
+def test_outputs_that_lie_on_themselves_are_refused():
+    from dihydrogen_amd.tokens import Attention, LayerNormalization, RotaryPositions
+    x = torch.ones(2, 3, 4, 8, device="cuda")
+    flat = torch.ones(2, 3, 1, 8, device="cuda").expand(2, 3, 4, 8)
+    with pytest.raises(ValueError):
+        Attention().forward(x, x, x, flat)
+    with pytest.raises(ValueError):
+        LayerNormalization().forward(x, None, None, flat)
+    with pytest.raises(ValueError):
+        RotaryPositions(8, [4]).forward(x, torch.zeros(1, 3, dtype=torch.int32, device="cuda"), flat)
+    o = torch.empty_like(x)
+    Attention().forward(flat, flat, flat, o)  # as inputs they are fine
+    assert bool((o == 1).all())
+
+
 def test_more_than_32_bits_of_offsets():
     """A cache of one sample whose last keys lie beyond 2^31 elements, and 2^32 bytes."""
     from dihydrogen_amd.tokens import Attention

@@ -39,7 +39,7 @@ def test_layer_norm():
     assert fwd(dtype=capi.F64, weights=capi.F32) == UNSUPPORTED and fwd(dtype=capi.F16, weights=capi.BF16) == UNSUPPORTED
     assert fwd(c=0) == INVALID and fwd(c=-3) == INVALID and fwd(eps=-1.0) == INVALID and fwd(eps=float("nan")) == INVALID
     assert fwd(mean=None) == INVALID and fwd(rstd=None) == INVALID and fwd(x=None) == INVALID and fwd(y=None) == INVALID
-    assert fwd(rows=1 << 31) == TOO_LARGE
+    assert fwd(rows=1 << 31) == TOO_LARGE and fwd(c=(1 << 26) + 1) == TOO_LARGE
     assert fwd(rows=0, x=None, y=None, mean=None, rstd=None) == 0
     assert fwd(xg=_geometry((8, 4), (1, 8))) > 0
     assert fwd(xg=_geometry((8, 5), (1, 8))) == INVALID  # not four rows
