@@ -52,6 +52,10 @@ struct Args
     int dim, query_heads, group;
     int blocks, heads; // of rows in a head, and heads in all samples
     Schedule schedule;
+    // The other side's tiles of a block of rows are shared by `parts` workgroups (1: one writes the gradients).  Part p's sums for row r, of `rows`, lie
+    // at (p * rows + r) * padded_dim, those for the values behind those for the keys.
+    int parts;
+    float* partials;
 };
 
 // dq, and what the other pass needs of each row.  As in the forward pass, the waves of a workgroup take 32 queries of a head each.
@@ -61,10 +65,11 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr int KT = kTileRows<T>, B = KT / 32;
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, KT>];
-    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks);
+    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks * a.parts);
     if (place.head >= a.heads)
         return;
-    const int block = place.block, n = place.head / a.query_heads, head = place.head - n * a.query_heads;
+    const int block = place.block / a.parts, part = place.block - block * a.parts;
+    const int n = place.head / a.query_heads, head = place.head - n * a.query_heads;
     const int lane = threadIdx.x & (kWaveSize - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const Sample sample = sample_of(a.masks, n);
 
@@ -79,6 +84,8 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
         to = sample.end_key(block_end - 1);
     }
     const int tiles = (max(to - from, 0) + KT - 1) / KT;
+    const int first_tile = static_cast<int>(static_cast<int64_t>(tiles) * part / a.parts);
+    const int end_tile = static_cast<int>(static_cast<int64_t>(tiles) * (part + 1) / a.parts);
     const T* const k = a.k + n * a.ks.sample + (head / a.group) * a.ks.head;
     const T* const v = a.v + n * a.vs.sample + (head / a.group) * a.vs.head;
     const int k_bytes = static_cast<int>(a.ks.token * sizeof(T)), v_bytes = static_cast<int>(a.vs.token * sizeof(T));
@@ -94,10 +101,10 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
         k_load.put((LdsBytes) lds[tile & 1][0], threadIdx.x);
         v_load.put((LdsBytes) lds[tile & 1][1], threadIdx.x);
     };
-    if (tiles > 0)
+    if (first_tile < end_tile)
     {
-        issue(0);
-        put(0);
+        issue(first_tile);
+        put(first_tile);
     }
 
     const int row_from = sample.first_key(min(i, max(last, 0))), row_end = sample.end_key(min(i, max(last, 0)));
@@ -126,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
         const float l = a.logsumexp[row];
         if (l > -INFINITY)
             log2_sum = l * kLog2e;
-        if (lane < 32)
+        if (lane < 32 && part == 0)
         {
             a.log2_sum[row] = log2_sum;
             a.delta[row] = delta;
@@ -139,11 +146,11 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
     const int some_from = sample.first_key(first), some_end = sample.end_key(last);
     const int all_from = sample.first_key(last), all_end = sample.end_key(first);
 
-    for (int tile = 0; tile < tiles; ++tile)
+    for (int tile = first_tile; tile < end_tile; ++tile)
     {
         wait_for_loads();
         __syncthreads();
-        if (tile + 1 < tiles)
+        if (tile + 1 < end_tile)
             issue(tile + 1);
         const LdsBytes k_tile = (LdsBytes) lds[tile & 1][0], v_tile = (LdsBytes) lds[tile & 1][1];
         const int at = from + tile * KT;
@@ -173,12 +180,17 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
             for (int b = 0; b < B; ++b)
                 accumulate<T, DP, KT>(k_tile, 32 * b, ds[b], dq);
         }
-        if (tile + 1 < tiles)
+        if (tile + 1 < end_tile)
             put(tile + 1); // (all waves are past the tile that lay there)
         if constexpr (kWavesOf<T, DP, Whole> == 1)
             keep_apart(dq);
     }
-    if (i < a.masks.queries)
+    if (i >= a.masks.queries)
+        return;
+    if (a.parts > 1)
+        store_row<float, DP, true>(
+            a.partials + (static_cast<int64_t>(part) * a.heads * a.masks.queries + row) * DP, DP, dq, 1.0f);
+    else
         store_row<T, DP, Whole>(a.dq + n * a.dqs.sample + head * a.dqs.head + i * a.dqs.token, a.dim, dq, a.scale);
 #endif
 }
@@ -194,10 +206,11 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, QT>];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kWaveSize];
     const int key_heads = a.query_heads / a.group;
-    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks);
+    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks * a.parts);
     if (place.head >= a.heads)
         return;
-    const int block = place.block, n = place.head / key_heads, key_head = place.head - n * key_heads;
+    const int block = place.block / a.parts, part = place.block - block * a.parts;
+    const int n = place.head / key_heads, key_head = place.head - n * key_heads;
     const int lane = threadIdx.x & (kWaveSize - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveSize);
     const Sample sample = sample_of(a.masks, n);
 
@@ -232,11 +245,13 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
         q_load.put((LdsBytes) lds[stage][0], threadIdx.x);
         d_o_load.put((LdsBytes) lds[stage][1], threadIdx.x);
     };
-    const int steps = tiles * a.group;
-    if (steps > 0)
+    const int64_t all_steps = static_cast<int64_t>(tiles) * a.group;
+    const int first_step = static_cast<int>(all_steps * part / a.parts), steps = static_cast<int>(all_steps * (part + 1) / a.parts);
+    int g = tiles > 0 ? first_step / tiles : 0, tile = first_step - g * tiles;
+    if (first_step < steps)
     {
-        issue(0, 0, 0);
-        put(0);
+        issue(g, tile, first_step & 1);
+        put(first_step & 1);
     }
 
     const int row_from = sample.first_query(min(j, max(last, 0))), row_end = sample.end_query(min(j, max(last, 0)));
@@ -251,8 +266,7 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
     const int some_from = sample.first_query(first), some_end = sample.end_query(last);
     const int all_from = sample.first_query(last), all_end = sample.end_query(first);
 
-    int g = 0, tile = 0;
-    for (int step = 0; step < steps; ++step)
+    for (int step = first_step; step < steps; ++step)
     {
         const int stage = step & 1, here = from + tile * QT;
         wait_for_loads();
@@ -315,10 +329,50 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
             for (int d = 0; d < DP / 32; ++d)
                 dk[d] = dv[d] = zero16();
         }
+        if (a.parts > 1)
+        {
+            const int64_t rows = static_cast<int64_t>(a.heads) * a.masks.keys;
+            float* const p = a.partials + (part * rows + static_cast<int64_t>(place.head) * a.masks.keys + j) * DP;
+            store_row<float, DP, true>(p, DP, dk, 1.0f);
+            store_row<float, DP, true>(p + a.parts * rows * DP, DP, dv, 1.0f);
+            return;
+        }
         store_row<T, DP, Whole>(a.dk + n * a.dks.sample + key_head * a.dks.head + j * a.dks.token, a.dim, dk, a.scale);
         store_row<T, DP, Whole>(a.dv + n * a.dvs.sample + key_head * a.dvs.head + j * a.dvs.token, a.dim, dv, 1.0f);
     }
 #endif
+}
+
+// Sums of the parts of gradients, in the parts' order: four elements of a row a thread.
+template <typename T>
+struct Sum
+{
+    const float* partials;
+    T* out[2]; // of grid.y
+    Strides strides[2];
+    float factor[2];
+    int parts, padded_dim, dim, tokens, heads; // heads of a sample
+    int64_t rows;
+};
+template <typename T>
+__global__ void __launch_bounds__(kThreads) attention_sum_kernel(const Sum<T> a)
+{
+    const int fours = a.padded_dim / 4, which = blockIdx.y;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x, row = at / fours;
+    const int d = static_cast<int>(at - row * fours) * 4;
+    if (row >= a.rows || d >= a.dim)
+        return;
+    const float* p = a.partials + (which * static_cast<int64_t>(a.parts) * a.rows + row) * a.padded_dim + d;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int part = 0; part < a.parts; ++part, p += a.rows * a.padded_dim)
+        sum += *reinterpret_cast<const f32x4*>(p);
+    const int64_t of_head = row / a.tokens, i = row - of_head * a.tokens, n = of_head / a.heads, head = of_head - n * a.heads;
+    T* const out = a.out[which] + n * a.strides[which].sample + head * a.strides[which].head + i * a.strides[which].token + d;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (d + e < a.dim)
+            out[e] = static_cast<T>(sum[e] * a.factor[which]);
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------
@@ -328,30 +382,94 @@ size_t rows_of(const h2x_attention& a)
     return static_cast<size_t>(a.samples) * a.query_heads * a.queries;
 }
 
-template <typename T, bool Whole>
-int issue(const h2x_attention& c, Args<T> a, hipStream_t stream)
+// How a call is run.
+struct Plan
 {
-    const int rows = kWaves * kRows;
-    const uint64_t query_blocks = (c.queries + rows - 1) / rows, key_blocks = (c.keys + rows - 1) / rows;
-    const uint64_t query_groups = query_blocks * c.samples * c.query_heads, key_groups = key_blocks * c.samples * c.key_heads;
+    uint64_t query_blocks, key_blocks; // of a head
+    int query_parts, key_parts;
+    size_t partials_bytes, bytes; // of the workspace: of the partial sums, and of all
+};
+
+// The other side's tiles in parts, while workgroups are fewer than CUs (twice as many under a mask that bounds one side, where they are of unlike
+// lengths), 16 tiles a part at least.  (Without and with parts, bf16: 8 query heads over one key head, 4096 tokens of 128, causal,
+// 1082 and 196 us; 16384 queries and 77 keys, 8 heads of 64, 370 and 57; 100 queries and 16384 keys, 2 heads, 276 and 36.)
+int parts_of(const h2x_attention& a, uint64_t groups, uint64_t tiles)
+{
+    const uint64_t most = ((a.window_left < 0) != (a.window_right < 0) ? 2 : 1) * static_cast<uint64_t>(chip_units());
+    int parts = 1;
+    while (parts < 64 && groups * parts * 2 <= most && tiles >= 32u * parts)
+        parts *= 2;
+    return parts;
+}
+
+Plan plan_of(const h2x_attention& a)
+{
+    const uint64_t rows = kWaves * kRows, tile = a.dtype == H2X_F32 ? 32 : 64;
+    Plan p{};
+    p.query_blocks = (a.queries + rows - 1) / rows;
+    p.key_blocks = (a.keys + rows - 1) / rows;
+    p.query_parts = parts_of(a, p.query_blocks * a.samples * a.query_heads, (a.keys + tile - 1) / tile);
+    p.key_parts = parts_of(a, p.key_blocks * a.samples * a.key_heads, (a.queries + tile - 1) / tile * (a.query_heads / a.key_heads));
+    const size_t dim = (a.head_dim + 31) / 32 * 32 * 4;
+    const size_t of_queries = p.query_parts > 1 ? p.query_parts * rows_of(a) * dim : 0;
+    const size_t of_keys = p.key_parts > 1 ? 2 * p.key_parts * static_cast<size_t>(a.samples) * a.key_heads * a.keys * dim : 0;
+    p.partials_bytes = of_queries > of_keys ? of_queries : of_keys; // (one after the other)
+    p.bytes = p.partials_bytes + 8 * rows_of(a);
+    return p;
+}
+
+template <typename T, bool Whole>
+int issue(const h2x_attention& c, const Plan& p, Args<T> a, hipStream_t stream)
+{
+    const uint64_t query_heads = static_cast<uint64_t>(c.samples) * c.query_heads, key_heads = static_cast<uint64_t>(c.samples) * c.key_heads;
+    const uint64_t query_groups = p.query_blocks * p.query_parts * query_heads, key_groups = p.key_blocks * p.key_parts * key_heads;
     if (query_groups > 0x800000u || key_groups > 0x800000u) // a grid of fewer than 2^32 threads
         return H2X_ERR_TOO_LARGE;
     const auto grid = [](uint64_t groups) { return dim3(static_cast<uint32_t>((groups + kNumXcd - 1) / kNumXcd * kNumXcd)); };
     return with_padded_dim(c.head_dim, [&](auto dim) {
         constexpr int DP = decltype(dim)::in_lds, DQ = decltype(dim)::contracted;
+        Sum<T> sum{a.partials, {}, {}, {a.scale, 1.0f}, 0, DP, c.head_dim, 0, 0, 0};
+        const auto join = [&](int outputs) {
+            launch(attention_sum_kernel<T>, dim3(static_cast<uint32_t>((sum.rows * (DP / 4) + kThreads - 1) / kThreads), outputs),
+                   dim3(kThreads), stream, sum);
+        };
         if (query_groups > 0)
         {
-            a.blocks = static_cast<int>(query_blocks);
-            a.heads = c.samples * c.query_heads;
-            a.schedule = schedule_of(c, false, a.heads, query_blocks);
+            a.blocks = static_cast<int>(p.query_blocks);
+            a.heads = static_cast<int>(query_heads);
+            a.parts = p.query_parts;
+            a.schedule = schedule_of(c, false, a.heads, p.query_blocks * p.query_parts);
             launch(attention_dq_kernel<T, DP, DQ, Whole>, grid(query_groups), dim3(kThreads), stream, a);
+            if (a.parts > 1)
+            {
+                sum.out[0] = a.dq;
+                sum.strides[0] = a.dqs;
+                sum.parts = a.parts;
+                sum.tokens = static_cast<int>(c.queries);
+                sum.heads = c.query_heads;
+                sum.rows = static_cast<int64_t>(rows_of(c));
+                join(1);
+            }
         }
         if (key_groups > 0)
         {
-            a.blocks = static_cast<int>(key_blocks);
-            a.heads = c.samples * c.key_heads;
-            a.schedule = schedule_of(c, true, a.heads, key_blocks);
+            a.blocks = static_cast<int>(p.key_blocks);
+            a.heads = static_cast<int>(key_heads);
+            a.parts = p.key_parts;
+            a.schedule = schedule_of(c, true, a.heads, p.key_blocks * p.key_parts);
             launch(attention_dkv_kernel<T, DP, DQ, Whole>, grid(key_groups), dim3(kThreads), stream, a);
+            if (a.parts > 1)
+            {
+                sum.out[0] = a.dk;
+                sum.out[1] = a.dv;
+                sum.strides[0] = a.dks;
+                sum.strides[1] = a.dvs;
+                sum.parts = a.parts;
+                sum.tokens = static_cast<int>(c.keys);
+                sum.heads = c.key_heads;
+                sum.rows = static_cast<int64_t>(key_heads) * c.keys;
+                join(2);
+            }
         }
         return launch_status();
     });
@@ -366,7 +484,9 @@ using namespace h2x::attention;
 
 extern "C" size_t h2x_attention_backward_workspace_bytes(const h2x_attention* attention)
 {
-    return check(attention) == H2X_SUCCESS ? 8 * rows_of(*attention) : 0;
+    if (check(attention) != H2X_SUCCESS || attention->samples == 0 || attention->query_heads == 0)
+        return 0;
+    return plan_of(*attention).bytes;
 }
 
 extern "C" int h2x_attention_backward(const h2x_attention* attention, const void* q, const void* k, const void* v, const void* o,
@@ -400,8 +520,11 @@ extern "C" int h2x_attention_backward(const h2x_attention* attention, const void
     }
     if (c.samples == 0 || c.query_heads == 0 || (c.queries == 0 && c.keys == 0))
         return H2X_SUCCESS;
-    if (missing || (c.queries > 0 && (!logsumexp || !workspace)))
+    const Plan p = plan_of(c);
+    if (missing || (c.queries > 0 && !logsumexp) || (p.bytes > 0 && !workspace))
         return H2X_ERR_INVALID_ARGUMENT;
+    if ((c.queries + 31) / 32 * (c.query_heads / c.key_heads) > 0x7fffffff)
+        return H2X_ERR_TOO_LARGE;
     return with_elements(c.dtype, whole, [&](auto t, auto is_whole) {
         using T = decltype(t);
         Args<T> a{};
@@ -414,7 +537,8 @@ extern "C" int h2x_attention_backward(const h2x_attention* attention, const void
         a.dq = static_cast<T*>(dq);
         a.dk = static_cast<T*>(dk);
         a.dv = static_cast<T*>(dv);
-        a.log2_sum = static_cast<float*>(workspace);
+        a.partials = static_cast<float*>(workspace);
+        a.log2_sum = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.partials_bytes);
         a.delta = a.log2_sum + rows_of(c);
         Strides* const strides[] = {&a.qs, &a.ks, &a.vs, &a.os, &a.d_os, &a.dqs, &a.dks, &a.dvs};
         for (int i = 0; i < 8; ++i)
@@ -425,6 +549,6 @@ extern "C" int h2x_attention_backward(const h2x_attention* attention, const void
         a.dim = c.head_dim;
         a.query_heads = c.query_heads;
         a.group = c.query_heads / c.key_heads;
-        return issue<T, decltype(is_whole)::value>(c, a, as_stream(stream));
+        return issue<T, decltype(is_whole)::value>(c, p, a, as_stream(stream));
     });
 }

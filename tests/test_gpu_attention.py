@@ -139,6 +139,19 @@ def test_keys_in_parts(dtype, queries, keys, heads, key_heads, n):
 
 
 @DTYPES
+@pytest.mark.parametrize("queries,keys,heads,key_heads,dim,n", [(2500, 100, 4, 1, 64, 1), (70, 4500, 2, 2, 40, 1), (1500, 1300, 8, 1, 128, 1),
+                                                                (1100, 1100, 3, 1, 72, 2)])
+def test_gradients_in_parts(dtype, queries, keys, heads, key_heads, dim, n):
+    """Few blocks of rows and many of the other side: shared out, and summed in order; some parts empty."""
+    for window, lengths in (((None, None), None), ((None, 0), None), ((200, 30), None),
+                            ((None, 0), ([max(1, queries - 90)] * n, [keys - 60] * n)), ((None, None), ([5] * n, [3] * n))):
+        p = Problem(n, queries, keys, heads, key_heads, dim, dtype, window=window, lengths=lengths, layout="gaps")
+        p.check()
+        first = [t[1].clone() for t in p.outputs[1:]]
+        assert all(torch.equal(a, b) for a, b in zip(first, p.backward()))
+
+
+@DTYPES
 @pytest.mark.parametrize("magnitude", [0.01, 30.0])
 def test_sharp_and_flat_rows(dtype, magnitude):
     """Scores of a few thousandths, and of hundreds: one key takes all."""
