@@ -1449,8 +1449,8 @@ typedef struct h2x_attention
     h2x_token_strides d_o, dq, dk, dv;    /* the backward pass alone */
 } h2x_attention;
 
-/** Bytes of workspace of h2x_attention_forward (0: none), without initialisation or state between calls; not for two calls that may
- * run at the same time. */
+/** Bytes of workspace of h2x_attention_forward (0: none), without initialisation or state between calls, aligned to 16 bytes; not for two
+ * calls that may run at the same time.  To be asked with the call's device as the current one: the way a call is run goes with its CUs. */
 size_t h2x_attention_forward_workspace_bytes(const h2x_attention* attention);
 
 /**
