@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
 {
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr bool kOneWave = DP == 128 || kWavesOf<T, DP, Whole> == 1; // (128 elements: two waves would have to spill)
-    constexpr int QT = kTileRows<T>, B = QT / 32;
+    constexpr int QT = kTileRows<T>, B = QT / 32, N = DP <= 64 ? 1 : B; // blocks at a time
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, QT>];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kWaveSize];
     const int key_heads = a.query_heads / a.group;
@@ -278,26 +278,30 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
         const LdsBytes q_tile = (LdsBytes) lds[stage][0], d_o_tile = (LdsBytes) lds[stage][1];
         const float* const log2_sum = &stats[stage][0][4 * (lane / 32)];
         const float* const delta = &stats[stage][1][4 * (lane / 32)];
-        if (first <= last && here < some_end && here + QT > some_from)
+#pragma unroll
+        for (int b0 = 0; b0 < B; b0 += N)
         {
+            const int at = here + 32 * b0;
+            if (first > last || at >= some_end || at + 32 * N <= some_from)
+                continue;
             // All blocks of the tile in one go: the products of one run beside the exponentials of another.
-            f32x16 s[B], dp[B];
-            products<T, DP, DQ, QT>(q_tile, 0, k, s);
-            products<T, DP, DQ, QT>(d_o_tile, 0, v, dp);
-            if (here < all_from || here + QT > all_end)
+            f32x16 s[N], dp[N];
+            products<T, DP, DQ, QT>(q_tile, 32 * b0, k, s);
+            products<T, DP, DQ, QT>(d_o_tile, 32 * b0, v, dp);
+            if (at < all_from || at + 32 * N > all_end)
             {
 #pragma unroll
-                for (int b = 0; b < B; ++b)
-                    hide(&s[b], here + 32 * b, row_from, row_end);
+                for (int b = 0; b < N; ++b)
+                    hide(&s[b], at + 32 * b, row_from, row_end);
             }
-            Weights<T> p[B], ds[B];
+            Weights<T> p[N], ds[N];
 #pragma unroll
-            for (int b = 0; b < B; ++b)
+            for (int b = 0; b < N; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; r += 4)
                 {
-                    const f32x4 l = *reinterpret_cast<const f32x4*>(log2_sum + 32 * b + 2 * r);
-                    const f32x4 m = *reinterpret_cast<const f32x4*>(delta + 32 * b + 2 * r);
+                    const f32x4 l = *reinterpret_cast<const f32x4*>(log2_sum + 32 * (b0 + b) + 2 * r);
+                    const f32x4 m = *reinterpret_cast<const f32x4*>(delta + 32 * (b0 + b) + 2 * r);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                     {
@@ -310,10 +314,10 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
                     ds[b].set(r + 2, dp[b][r + 2], dp[b][r + 3]);
                 }
 #pragma unroll
-            for (int b = 0; b < B; ++b)
+            for (int b = 0; b < N; ++b)
             {
-                accumulate<T, DP, QT>(d_o_tile, 32 * b, p[b], dv);
-                accumulate<T, DP, QT>(q_tile, 32 * b, ds[b], dk);
+                accumulate<T, DP, QT>(d_o_tile, 32 * (b0 + b), p[b], dv);
+                accumulate<T, DP, QT>(q_tile, 32 * (b0 + b), ds[b], dk);
             }
         }
         if (step + 1 < steps)
