@@ -524,6 +524,10 @@ extern "C" int h2x_attention_backward(const h2x_attention* attention, const void
     }
     if (c.samples == 0 || c.query_heads == 0 || (c.queries == 0 && c.keys == 0))
         return H2X_SUCCESS;
+    for (int out = 5; out < 8; ++out) // the second kernel reads what the first would have overwritten
+        for (int x = 0; x < out; ++x)
+            if (operands[out].p && operands[out].p == operands[x].p)
+                return H2X_ERR_INVALID_ARGUMENT;
     const Plan p = plan_of(c);
     if (missing || (c.queries > 0 && !logsumexp) || (p.bytes > 0 && !workspace))
         return H2X_ERR_INVALID_ARGUMENT;

@@ -526,7 +526,7 @@ extern "C" int h2x_attention_forward(const h2x_attention* attention, const void*
     if (rows_of(c) == 0)
         return H2X_SUCCESS;
     const Plan p = plan_of(c);
-    if (!q || !o || (c.keys > 0 && (!k || !v)) || (p.parts > 1 && !workspace))
+    if (!q || !o || (c.keys > 0 && (!k || !v || o == k || o == v)) || (p.parts > 1 && !workspace))
         return H2X_ERR_INVALID_ARGUMENT;
     if (p.groups > 0x800000u || (p.parts > 1 && rows_of(c) > 0x800000u))
         return H2X_ERR_TOO_LARGE; // (a grid of fewer than 2^32 threads)

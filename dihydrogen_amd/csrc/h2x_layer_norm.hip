@@ -721,7 +721,7 @@ extern "C" int h2x_layer_norm_forward(h2x_dtype dtype, h2x_dtype weight_dtype, s
             return H2X_ERR_INVALID_ARGUMENT;
         if (num_rows == 0)
             return H2X_SUCCESS;
-        if (!x || !y)
+        if (!x || !y || (x == y && !alike(a.x_rows, a.y_rows)))
             return H2X_ERR_INVALID_ARGUMENT;
         a.num_rows = static_cast<uint32_t>(num_rows);
         a.channels = num_channels;
@@ -762,6 +762,8 @@ extern "C" int h2x_layer_norm_backward(h2x_dtype dtype, h2x_dtype weight_dtype, 
             || !make_rows(dx_rows, num_rows, num_channels, &a.dx_rows))
             return H2X_ERR_INVALID_ARGUMENT;
         if ((weights && !workspace) || (num_rows > 0 && (!x || !dy || !mean || !rstd)))
+            return H2X_ERR_INVALID_ARGUMENT;
+        if (dx && ((dx == x && !alike(a.dx_rows, a.x_rows)) || (dx == dy && !alike(a.dx_rows, a.dy_rows))))
             return H2X_ERR_INVALID_ARGUMENT;
         if (!weights && (!dx || num_rows == 0))
             return H2X_SUCCESS;

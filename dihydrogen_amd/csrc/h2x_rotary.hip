@@ -226,6 +226,9 @@ extern "C" int h2x_rotary_apply(const h2x_rotary* rotary, const void* x, const i
         return H2X_SUCCESS;
     if (!x || !y || (pairs > 0 && (!positions || !frequencies)))
         return H2X_ERR_INVALID_ARGUMENT;
+    if (x == y && ((r.samples > 1 && r.x.sample != r.y.sample) || (r.tokens > 1 && r.x.token != r.y.token)
+                   || (r.heads > 1 && r.x.head != r.y.head)))
+        return H2X_ERR_INVALID_ARGUMENT;
     a.positions = positions;
     a.frequencies = frequencies;
     a.positions_sample_stride = r.positions_sample_stride;

@@ -47,6 +47,17 @@ struct Rows
     int num; // 0: rows one after another, stride[0] apart
 };
 
+// Whether two tensors' rows lie alike.
+inline bool alike(const Rows& a, const Rows& b)
+{
+    if (a.num != b.num || a.stride[0] != b.stride[0])
+        return false;
+    for (int d = 0; d < a.num; ++d)
+        if (a.stride[d] != b.stride[d] || a.extent[d].divisor != b.extent[d].divisor)
+            return false;
+    return true;
+}
+
 #ifdef __HIPCC__
 __device__ __forceinline__ int64_t row_offset(const Rows& rows, uint32_t r)
 {

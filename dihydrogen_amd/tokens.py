@@ -197,7 +197,7 @@ def grid_positions(tensor: Tensor, dims: Optional[Sequence[int]] = None) -> torc
 class RotaryPositions:
     """Turns pairs of a head's elements by angles that grow with a token's position: pair i of an axis
     with m pairs by position * base ** (-i / m).  ``axis_pairs``: how many pairs belong to each axis (time or depth, height, width); elements
-    behind the pairs are copied.
+    behind the pairs are copied.  ``frequencies``, a float64 tensor of one a pair, may be replaced before the first call.
 
     x: (samples, tokens, heads, head_dim), float32, float64, bfloat16 or float16.  positions: int32, (axes, tokens) for all
     samples or (samples, axes, tokens), tokens contiguous; see grid_positions().

@@ -28,7 +28,7 @@ def _geometry(shape, strides):
 
 def test_layer_norm():
     lib = capi.load()
-    F, B = lib.h2x_layer_norm_forward, lib.h2x_layer_norm_backward
+    F, B, O = lib.h2x_layer_norm_forward, lib.h2x_layer_norm_backward, ctypes.c_void_p(2 << 20)
 
     def fwd(dtype=capi.F32, weights=capi.F32, rows=4, c=8, xg=None, yg=None, x=P, y=P, mean=P, rstd=P, eps=1e-5):
         return F(dtype, weights, rows, c, xg, yg, x, P, P, y, mean, rstd, eps, None)
@@ -42,6 +42,9 @@ def test_layer_norm():
     assert fwd(rows=1 << 31) == TOO_LARGE and fwd(c=(1 << 26) + 1) == TOO_LARGE
     assert fwd(rows=0, x=None, y=None, mean=None, rstd=None) == 0
     assert fwd(xg=_geometry((8, 4), (1, 8))) > 0
+    assert fwd(xg=_geometry((8, 4), (1, 16))) == INVALID  # in place, but laid out otherwise
+    assert fwd(xg=_geometry((8, 4), (1, 16)), y=ctypes.c_void_p(2 << 20)) > 0
+    assert B(capi.F32, capi.F32, 4, 8, None, _geometry((8, 4), (1, 16)), None, P, O, P, P, P, O, None, None, None, None) == INVALID
     assert fwd(xg=_geometry((8, 5), (1, 8))) == INVALID  # not four rows
     assert fwd(xg=_geometry((7, 4), (1, 8))) == INVALID and fwd(yg=_geometry((8, 4), (2, 8))) == INVALID
     assert fwd(xg=_geometry((8, 4, -1), (1, 8, 8))) == INVALID
@@ -63,7 +66,7 @@ def _rotary(**changes):
         if name == "axis_pairs":
             r.axis_pairs[:len(value)] = value
         else:
-            setattr(r, name, value)
+            setattr(r, name.split("_strides")[0], value)
     return r
 
 
@@ -81,6 +84,8 @@ def test_rotary():
     assert call(num_axes=5) == INVALID and call(num_axes=-1) == INVALID and call(pairing=2) == INVALID
     assert call(heads=-1) == INVALID and call(samples=-1) == INVALID and call(tokens=-1) == INVALID
     assert call(tokens=1 << 31) == TOO_LARGE
+    assert call(y_strides=capi.TokenStrides(48, 8, 24)) == INVALID  # in place, but laid out otherwise
+    assert call(y_strides=capi.TokenStrides(48, 8, 24), y=ctypes.c_void_p(2 << 20)) > 0
     assert call(x=None) == INVALID and call(y=None) == INVALID and call(positions=None) == INVALID and call(frequencies=None) == INVALID
     assert call(tokens=0, x=None, y=None) == 0 and call(heads=0) == 0 and call(samples=0) == 0
 
@@ -100,14 +105,16 @@ def _attention(**changes):
 def test_attention():
     lib = capi.load()
 
-    def fwd(q=P, k=P, v=P, o=P, ws=None, **changes):
+    O, A, B, C = (ctypes.c_void_p(i << 20) for i in (2, 3, 4, 5))
+
+    def fwd(q=P, k=P, v=P, o=O, ws=None, **changes):
         return lib.h2x_attention_forward(ctypes.byref(_attention(**changes)), q, k, v, None, None, o, P, ws, None)
 
-    def bwd(q=P, lse=P, dq=P, dv=P, ws=P, **changes):
-        return lib.h2x_attention_backward(ctypes.byref(_attention(**changes)), q, P, P, P, P, lse, None, None, dq, P, dv, ws, None)
+    def bwd(q=P, lse=P, dq=A, dv=B, ws=P, **changes):
+        return lib.h2x_attention_backward(ctypes.byref(_attention(**changes)), q, P, P, P, P, lse, None, None, dq, C, dv, ws, None)
 
     for call in (fwd, bwd):
-        assert call() > 0
+        assert call() > 0, call
         assert call(dtype=capi.F16) == UNSUPPORTED and call(dtype=capi.F64) == UNSUPPORTED and call(dtype=9) == UNSUPPORTED
         assert call(head_dim=129) == UNSUPPORTED and call(head_dim=0) == INVALID
         assert call(key_heads=3) == INVALID and call(key_heads=0) == INVALID and call(samples=-1) == INVALID
@@ -121,11 +128,20 @@ def test_attention():
         assert call(queries=0, keys=0) == 0 and call(samples=0) == 0 and call(query_heads=0, key_heads=0) == 0
     assert lib.h2x_attention_forward(None, P, P, P, None, None, P, P, None, None) == INVALID
     assert fwd(o=None) == INVALID
-    assert fwd(o=P) > 0
+    assert fwd(o=O) > 0 and fwd(o=P) == INVALID
     a = _attention()
     a.o = capi.TokenStrides(4 * 64, 4 * 64, 32)  # heads of the output on one another
     assert lib.h2x_attention_forward(ctypes.byref(a), P, P, P, None, None, P, P, None, None) == INVALID
     assert bwd(lse=None) == INVALID and bwd(dq=None) == INVALID and bwd(dv=None) == INVALID and bwd(ws=None) == INVALID
+    # outputs where inputs or other outputs lie
+    others = [ctypes.c_void_p((i + 2) << 20) for i in range(8)]
+    run = lambda p: lib.h2x_attention_backward(ctypes.byref(_attention()), *p[:5], P, None, None, *p[5:], P, None)
+    assert run(others) > 0
+    for out in (5, 6, 7):
+        for other in range(8):
+            if other != out:
+                assert run([others[other] if i == out else p for i, p in enumerate(others)]) == INVALID
+    assert lib.h2x_attention_forward(ctypes.byref(_attention()), others[0], P, others[1], None, None, P, None, None, None) == INVALID
     # keys in parts need a workspace
     long = _attention(queries=1, keys=1 << 17, samples=1)
     for name in ("k", "v"):
