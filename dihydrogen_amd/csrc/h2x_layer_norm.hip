@@ -21,16 +21,38 @@ template <int Threads, int Vectors>
 struct Shape
 {
     static constexpr int threads = Threads, vectors = Vectors;
-    static constexpr bool wave_rows = Threads == kWaveSize; // a workgroup's waves have rows of their own
+    static constexpr bool wave_rows = Threads <= kWaveSize; // a workgroup's waves have rows of their own, one or several at a time
+    static constexpr int rows_of_wave = wave_rows ? kWaveSize / Threads : 1;
     static constexpr int most_threads = wave_rows ? kBlockSize : Threads;
 };
+
+// Sum over each G lanes of a wave, a power of two from 8 on; all of them get it.
+template <int G, typename W>
+__device__ __forceinline__ W group_total(W v)
+{
+    constexpr int kHalfMirror = 0x141; // lane i of eight and lane 7 - i
+    const auto add = [](W a, W b) { return a + b; };
+    if constexpr (G == 64)
+        return wave_total(v);
+    if constexpr (G == 32)
+        v = combine_apart<16>(v, add);
+    if constexpr (G >= 16)
+    {
+        v += dpp_move<kDppRowRor8>(v);
+        v += dpp_move<kDppRowRor4>(v); // lanes 8 apart hold the same
+    }
+    else
+        v += dpp_move<kHalfMirror>(v);
+    v += dpp_move<kDppQuadSwap2>(v);
+    return v + dpp_move<kDppQuadSwap1>(v);
+}
 
 // Sum over the Threads of a row; all of them get it.  lds: one place a wave, of which two sets alternate between sums, so
 // that a barrier a sum is enough.
 template <int Threads, typename W>
 __device__ __forceinline__ W row_total(W v, W* lds)
 {
-    v = wave_total(v);
+    v = group_total<(Threads < kWaveSize ? Threads : kWaveSize)>(v);
     if constexpr (Threads > kWaveSize)
     {
         if ((threadIdx.x & (kWaveSize - 1)) == 0)
@@ -144,11 +166,11 @@ __global__ void __launch_bounds__(S::most_threads) ln_forward_kernel(const Forwa
     using W = wide<T>;
     constexpr int V = kVec<T>, K = S::vectors;
     constexpr bool kAhead = K * V <= 16;
-    __shared__ W lds[2][2][S::threads / kWaveSize];
-    const uint32_t waves = S::wave_rows ? blockDim.x / kWaveSize : 1;
-    const uint32_t step = gridDim.x * waves;
-    uint32_t r = blockIdx.x * waves + (S::wave_rows ? threadIdx.x / kWaveSize : 0);
-    const int t = S::wave_rows ? threadIdx.x & (kWaveSize - 1) : threadIdx.x, c = a.channels;
+    __shared__ W lds[2][2][S::wave_rows ? 1 : S::threads / kWaveSize];
+    const uint32_t at_once = S::wave_rows ? blockDim.x / S::threads : 1; // rows
+    const uint32_t step = gridDim.x * at_once;
+    uint32_t r = blockIdx.x * at_once + (S::wave_rows ? threadIdx.x / S::threads : 0);
+    const int t = threadIdx.x % S::threads, c = a.channels;
     if (r >= a.num_rows)
         return;
     UVec<T, V> x[K], next[kAhead ? K : 1];
@@ -300,20 +322,19 @@ struct Backward
     bool streamed; // dx
 };
 
-// Rows in registers, as in the forward pass.  A thread keeps the sums for the gradients of its columns' weights; the sums of waves with rows of their own
-// meet in LDS at the end, in the waves' order.
+// Rows in registers, as in the forward pass.  A thread keeps the sums for the gradients of its columns' weights; the sums of a workgroup's
+// rows at a time meet in LDS at the end, in order.
 template <typename T, typename P, typename S, bool Weights>
 __global__ void __launch_bounds__(S::most_threads) ln_backward_kernel(const Backward<T, P> a)
 {
     using W = wide<T>;
     constexpr int V = kVec<T>, K = S::vectors;
     constexpr bool kAhead = K * V <= 16;
-    constexpr int kWaves = S::wave_rows ? kWavesPerBlock : 1; // with rows of their own
-    __shared__ W lds[2][2][S::threads / kWaveSize];
-    const int wave = threadIdx.x / kWaveSize;
-    const int t = S::wave_rows ? threadIdx.x & (kWaveSize - 1) : threadIdx.x, c = a.channels;
-    const uint64_t step = static_cast<uint64_t>(gridDim.x) * kWaves;
-    uint64_t r = static_cast<uint64_t>(blockIdx.x) * kWaves + (S::wave_rows ? wave : 0);
+    constexpr int kAtOnce = S::wave_rows ? kBlockSize / S::threads : 1; // rows
+    __shared__ W lds[2][2][S::wave_rows ? 1 : S::threads / kWaveSize];
+    const int t = threadIdx.x % S::threads, group = threadIdx.x / S::threads, c = a.channels;
+    const uint64_t step = static_cast<uint64_t>(gridDim.x) * kAtOnce;
+    uint64_t r = static_cast<uint64_t>(blockIdx.x) * kAtOnce + group;
     W dscale[Weights ? K : 1][V], dbias[Weights ? K : 1][V];
     if constexpr (Weights)
     {
@@ -401,7 +422,7 @@ __global__ void __launch_bounds__(S::most_threads) ln_backward_kernel(const Back
         const size_t half = static_cast<size_t>(gridDim.x) * c;
         if constexpr (S::wave_rows)
         {
-            __shared__ W sums[kWaves - 1][kWaveSize * V];
+            __shared__ W sums[kAtOnce - 1][S::threads * V];
 #pragma unroll
             for (int k = 0; k < K; ++k)
 #pragma unroll
@@ -409,21 +430,21 @@ __global__ void __launch_bounds__(S::most_threads) ln_backward_kernel(const Back
                 {
                     W(&mine)[V] = which ? dbias[k] : dscale[k];
                     __syncthreads();
-                    if (wave > 0)
+                    if (group > 0)
                     {
 #pragma unroll
                         for (int i = 0; i < V; ++i)
-                            sums[wave - 1][i * kWaveSize + t] = mine[i];
+                            sums[group - 1][i * S::threads + t] = mine[i];
                     }
                     __syncthreads();
-                    const int at = (k * kWaveSize + t) * V;
-                    if (wave == 0 && at < c)
+                    const int at = (k * S::threads + t) * V;
+                    if (group == 0 && at < c)
                     {
 #pragma unroll
-                        for (int i = 0; i < V; ++i)
+                        for (int n = 0; n < kAtOnce - 1; ++n)
 #pragma unroll
-                            for (int n = 0; n < kWaves - 1; ++n)
-                                mine[i] += sums[n][i * kWaveSize + t];
+                            for (int i = 0; i < V; ++i)
+                                mine[i] += sums[n][i * S::threads + t];
                         store(out + which * half, at, c, mine, a.streamed);
                     }
                 }
@@ -558,26 +579,32 @@ __global__ void __launch_bounds__(kSumColumns* kSumLanes)
 
 constexpr int kMostChannels = 1 << 26; // a grid of fewer than 2^32 threads for the weights' sums
 
-// How the rows are shared out: the fewest threads whose registers hold a row, at 128 bytes of sums' type a thread, or 96 where a
-// workgroup of 512 threads leaves each 256 registers (the backward pass keeps four numbers an element).
+// How the rows are shared out: the fewest threads whose registers hold a row, one vector a thread below a wave, and 96 bytes of the sums' type a
+// thread from there on, 64 in workgroups of 256 (the backward pass keeps four numbers an element, and the next row).  (Forward and backward
+// in bf16, us, with a wave for rows of up to 2048 and 256 threads of up to 8192: 200000 x 32 62 and 169, 100000 x 300 37 and 104, 8192 x 2048
+// 18 and 47, 4096 x 8192 26 and 83; so 11 and 26, 37 and 68, 17 and 34, 27 and 64.)
 struct Split
 {
     int threads, vectors; // of a row; threads = 0: too long for registers
 };
 constexpr int most_vectors(int vec, int threads)
 {
-    return (threads == 512 ? 96 : 128) / (vec == 2 ? 8 : 4) / vec;
+    return threads < 64 ? 1 : (threads == 256 ? 64 : 96) / (vec == 2 ? 8 : 4) / vec;
 }
 Split split_rows(int vec, int channels)
 {
     const int64_t vectors = (static_cast<int64_t>(channels) + vec - 1) / vec;
-    for (const int threads : {64, 256, 512})
+    for (const int threads : {8, 16, 32, 64, 256, 512})
     {
         const int64_t each = (vectors + threads - 1) / threads;
         if (each <= most_vectors(vec, threads))
             return {threads, static_cast<int>(each)};
     }
     return {0, 0};
+}
+constexpr int rows_at_once(int threads)
+{
+    return threads == 0 || threads > kWaveSize ? 1 : kBlockSize / threads;
 }
 
 // Outputs from 16 MiB on go past the caches, which keep the inputs: x is read by the backward pass again.  (Forward and backward of
@@ -588,11 +615,12 @@ bool is_streamed(size_t rows, int channels, size_t size)
     return rows * channels * size >= size_t(16) << 20;
 }
 
-// Workgroups whose sums for the weights' gradients are added up at the end: two for each CU where rows are that many.
-uint32_t weight_parts(int threads, size_t num_rows)
+// Workgroups whose sums for the weights' gradients are added up at the end: two for each CU where rows are that many, four where
+// rows of a vector a thread leave registers for them.
+uint32_t weight_parts(const Split& s, size_t num_rows)
 {
-    const size_t rows_at_once = threads == 64 ? kWavesPerBlock : 1;
-    const size_t most = 2 * 256, groups = (num_rows + rows_at_once - 1) / rows_at_once;
+    const size_t most = (s.threads > 0 && s.threads <= kWaveSize && s.vectors == 1 ? 4 : 2) * 256;
+    const size_t groups = (num_rows + rows_at_once(s.threads) - 1) / rows_at_once(s.threads);
     return static_cast<uint32_t>(groups < most ? (groups ? groups : 1) : most);
 }
 
@@ -617,7 +645,10 @@ int with_vectors(int vectors, const F& f)
 template <int V, typename F>
 int with_shape(const Split& s, const F& f)
 {
-    return s.threads == 64    ? with_vectors<V, 64, 1>(s.vectors, f)
+    return s.threads == 8     ? f(Shape<8, 1>())
+           : s.threads == 16  ? f(Shape<16, 1>())
+           : s.threads == 32  ? f(Shape<32, 1>())
+           : s.threads == 64  ? with_vectors<V, 64, 1>(s.vectors, f)
            : s.threads == 256 ? with_vectors<V, 256, most_vectors(V, 64) / 4 + 1>(s.vectors, f)
                               : with_vectors<V, 512, most_vectors(V, 256) / 2 + 1>(s.vectors, f);
 }
@@ -634,8 +665,9 @@ int forward(const Forward<T, P>& a, hipStream_t stream)
     return with_shape<kVec<T>>(s, [&](auto shape) {
         using S = decltype(shape);
         // a wave's rows: four waves a workgroup, one where rows are fewer than the waves that run at once
-        const uint32_t waves = !S::wave_rows || a.num_rows <= 4 * chip_units() ? 1 : kWavesPerBlock;
-        launch(ln_forward_kernel<T, P, S>, dim3(workgroups(a.num_rows, waves, S::threads * waves)), dim3(S::threads * waves), stream, a);
+        const uint32_t waves = !S::wave_rows ? S::threads / kWaveSize : a.num_rows <= 4 * chip_units() ? 1 : kWavesPerBlock;
+        const uint32_t rows = S::wave_rows ? waves * S::rows_of_wave : 1;
+        launch(ln_forward_kernel<T, P, S>, dim3(workgroups(a.num_rows, rows, waves * kWaveSize)), dim3(waves * kWaveSize), stream, a);
         return launch_status();
     });
 }
@@ -645,7 +677,7 @@ int backward(const Backward<T, P>& a, P* dscale, P* dbias, hipStream_t stream)
 {
     const Split s = split_rows(kVec<T>, a.channels);
     const bool weights = dscale || dbias;
-    const uint32_t parts = weight_parts(s.threads, a.num_rows);
+    const uint32_t parts = weight_parts(s, a.num_rows);
     if (s.threads == 0)
     {
         if (weights) // first: dx may lie where x or dy does
@@ -665,7 +697,7 @@ int backward(const Backward<T, P>& a, P* dscale, P* dbias, hipStream_t stream)
             if (weights)
                 launch(ln_backward_kernel<T, P, S, true>, dim3(parts), dim3(kThreads), stream, a);
             else
-                launch(ln_backward_kernel<T, P, S, false>, dim3(workgroups(a.num_rows, S::wave_rows ? kWavesPerBlock : 1, kThreads)),
+                launch(ln_backward_kernel<T, P, S, false>, dim3(workgroups(a.num_rows, rows_at_once(S::threads), kThreads)),
                        dim3(kThreads), stream, a);
             return 0;
         });
@@ -736,7 +768,7 @@ extern "C" size_t h2x_layer_norm_workspace_bytes(h2x_dtype dtype, size_t num_row
     const int size = element_size(dtype);
     if (size == 0 || num_channels < 1)
         return 0;
-    const uint32_t parts = weight_parts(split_rows(16 / size, num_channels).threads, num_rows);
+    const uint32_t parts = weight_parts(split_rows(16 / size, num_channels), num_rows);
     return 2 * static_cast<size_t>(parts) * num_channels * (size == 8 ? 8 : 4);
 }
 

@@ -58,6 +58,13 @@ def test_against_the_plain_form(types, channels):
         assert ref.outside_untouched(yb, y, fill) and ref.outside_untouched(dxb, dx, fill)
 
 
+@pytest.mark.parametrize("types", TYPES, ids=lambda t: "-".join(str(x).split(".")[1] for x in t))
+@pytest.mark.parametrize("channels", [16, 17, 33, 100, 128, 130, 300, 700, 1500, 6145, 12000, 12289])
+def test_rows_of_every_share(types, channels):
+    """Rows that 8, 16 and 32 lanes hold, several to a wave, and those around the other shares' ends."""
+    test_against_the_plain_form(types, channels)
+
+
 @pytest.mark.parametrize("channels", [24, 40, 1155, 9001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
 def test_rows_apart(dtype, channels):
