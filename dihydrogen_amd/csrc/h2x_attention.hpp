@@ -597,7 +597,7 @@ inline int check(const h2x_attention* a)
     if (a->head_dim < 1 || a->samples < 0 || a->query_heads < 0 || a->key_heads < 0 || a->queries < 0 || a->keys < 0
         || (a->query_heads > 0 && (a->key_heads < 1 || a->query_heads % a->key_heads != 0)))
         return H2X_ERR_INVALID_ARGUMENT;
-    if (!(a->scale > 0) || !(a->scale <= 1e30))
+    if (!(a->scale >= 1e-30) || !(a->scale <= 1e30)) // (in 32 bits neither zero, which an infinite score would make NaN, nor infinite)
         return H2X_ERR_INVALID_ARGUMENT;
     if (a->head_dim > 128)
         return H2X_ERR_UNSUPPORTED;

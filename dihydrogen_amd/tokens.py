@@ -283,7 +283,7 @@ class Attention:
                  window: Tuple[Optional[int], Optional[int]] = (None, None), stream: Optional[torch.cuda.Stream] = None):
         left, right = window
         _require(all(w is None or w >= 0 for w in (left, right)), "a window reaches zero or more keys to either side")
-        _require(scale is None or 0 < scale < math.inf, "scale has to be positive")
+        _require(scale is None or 1e-30 <= scale <= 1e30, "scale has to be positive, from 1e-30 to 1e30")
         if causal:
             _require(right in (None, 0), "a causal window has no keys behind a query's place")
             right = 0

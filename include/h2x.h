@@ -1444,7 +1444,7 @@ typedef struct h2x_attention
     int32_t samples, query_heads, key_heads, reserved;
     int64_t queries, keys; /* below 2^31 */
     int64_t window_left, window_right;
-    double scale;
+    double scale; /* 1e-30 to 1e30 */
     h2x_token_strides q, k, v, o;         /* token strides of at least head_dim elements */
     h2x_token_strides d_o, dq, dk, dv;    /* the backward pass alone */
 } h2x_attention;

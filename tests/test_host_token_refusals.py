@@ -221,3 +221,16 @@ def test_positions_of_a_shard():
     at = (2 * h + 1) * w + 2  # plane 2, row 1, column 2 of the shard
     assert p[:, at].tolist() == [2, t.global_index[1] + 1, t.global_index[0] + 2]
     assert grid_positions(t, [0]).tolist() == [list(range(t.global_index[0], 7))]
+
+
+def test_scales_that_32_bits_do_not_hold():
+    from dihydrogen_amd.tokens import Attention
+    lib = capi.load()
+    for scale, status in ((1e-60, INVALID), (9e-31, INVALID), (1e-30, 0), (1e30, 0), (2e30, INVALID)):
+        a = _attention(scale=scale, samples=0)  # (nothing to launch)
+        assert lib.h2x_attention_forward(ctypes.byref(a), P, P, P, None, None, ctypes.c_void_p(2 << 20), P, None, None) == status
+        if status:
+            with pytest.raises(ValueError):
+                Attention(scale=scale)
+        else:
+            Attention(scale=scale)
