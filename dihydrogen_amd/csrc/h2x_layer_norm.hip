@@ -577,7 +577,7 @@ __global__ void __launch_bounds__(kSumColumns* kSumLanes)
 
 // ---- host ----------------------------------------------------------------------
 
-constexpr int kMostChannels = 1 << 26; // a grid of fewer than 2^32 threads for the weights' sums
+constexpr int kMostChannels = 1 << 25; // (the weights' sums take 64 threads a channel, and a grid fewer than 2^32)
 
 // How the rows are shared out: the fewest threads whose registers hold a row, one vector a thread below a wave, and 96 bytes of the sums' type a
 // thread from there on, 64 in workgroups of 256 (the backward pass keeps four numbers an element, and the next row).  (Forward and backward

@@ -1330,7 +1330,7 @@ int h2x_shuffle_direct(const h2x_shuffle_direct_plan* plan, void* const* src, vo
  * of 1 to H2X_MAX_DIMS dimensions with local_shape[0] == num_channels, strides[0] == 1 and num_rows as
  * the product of the other extents, r counting through them innermost first (the interior of a
  * haloed tensor whose channel is innermost).  y may be x itself, with the same rows.  Sums are in 32 bits (64
- * with H2X_F64), the squares' about the mean.  num_rows up to 2^31 - 1, num_channels up to 2^26.
+ * with H2X_F64), the squares' about the mean.  num_rows up to 2^31 - 1, num_channels up to 2^25.
  */
 int h2x_layer_norm_forward(h2x_dtype dtype,
                            h2x_dtype weight_dtype,

@@ -234,3 +234,13 @@ def test_scales_that_32_bits_do_not_hold():
                 Attention(scale=scale)
         else:
             Attention(scale=scale)
+
+
+def test_most_channels():
+    """The sums of the weights' gradients take 64 threads a channel, of fewer than 2^32."""
+    lib = capi.load()
+    most, O = 1 << 25, ctypes.c_void_p(2 << 20)
+    fwd = lambda c: lib.h2x_layer_norm_forward(capi.F32, capi.F32, 1, c, None, None, P, P, P, O, P, P, 1e-5, None)
+    bwd = lambda c: lib.h2x_layer_norm_backward(capi.F32, capi.F32, 1, c, None, None, None, P, P, P, P, P, O, P, P, P, None)
+    for call in (fwd, bwd):
+        assert call(most) > 0 and call(most + 1) == TOO_LARGE and call(1 << 26) == TOO_LARGE
