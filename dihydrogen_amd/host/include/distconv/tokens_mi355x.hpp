@@ -6,16 +6,40 @@
 // the C ABI, whose element types include the 16-bit ones that no tensor here has.
 //
 // As with the other layers calls are asynchronous on the backend's stream, and an object
-// keeps the workspace of its calls: one object is not for two streams at a time.
+// keeps the workspace of its calls: one object is not for two streams, nor for two graphs that run at a time.
 #pragma once
 
 #include "distconv/layers_mi355x.hpp"
 
+#include <algorithm>
 #include <cmath>
+#include <list>
 #include <vector>
 
 namespace distconv
 {
+
+// A layer's workspace.  One that has become too small is kept until the layer goes: graphs that were captured with it hold its address.  (Each is half as
+// large again as the one before at least, so that all of them are three times the last at most.)
+class TokenWorkspace
+{
+public:
+    void* get(size_t bytes)
+    {
+        if (bytes == 0)
+            return nullptr;
+        const size_t last = m_all.empty() ? 0 : m_all.back().get_size();
+        if (last < bytes)
+        {
+            m_all.emplace_back();
+            m_all.back().allocate(std::max(bytes, last + last / 2));
+        }
+        return m_all.back().get();
+    }
+
+private:
+    std::list<tensor::Memory<tensor::CUDAAllocator>> m_all;
+};
 
 template <typename Backend>
 class LayerNormalization;
@@ -48,12 +72,10 @@ public:
     {
         const h2x_tensor_geometry x = rows_of(input), dy = rows_of(d_output), dx = rows_of(d_input);
         const h2x_dtype type = Tensor::h2x_type();
-        const size_t need = h2x_layer_norm_workspace_bytes(type, num_rows(x), channels(x));
-        if (m_workspace.is_null() || m_workspace.get_size() < need)
-            m_workspace.allocate(need);
+        void* const workspace = m_workspace.get(d_scale || d_bias ? h2x_layer_norm_workspace_bytes(type, num_rows(x), channels(x)) : 0);
         DISTCONV_CHECK_H2X(h2x_layer_norm_backward(type, type, num_rows(x), channels(x), &x, &dy, &dx, input.get_const_base_ptr(),
                                                    d_output.get_const_base_ptr(), mean, rstd, scale, d_input.get_base_ptr(),
-                                                   d_scale, d_bias, m_workspace.get(), m_stream));
+                                                   d_scale, d_bias, workspace, m_stream));
         return 0;
     }
 
@@ -82,7 +104,7 @@ private:
 
     hipStream_t m_stream;
     double m_epsilon;
-    tensor::Memory<tensor::CUDAAllocator> m_workspace;
+    TokenWorkspace m_workspace;
 };
 
 template <typename Backend>
@@ -145,7 +167,7 @@ public:
                 const int32_t* query_lengths = nullptr, const int32_t* key_lengths = nullptr)
     {
         DISTCONV_CHECK_H2X(h2x_attention_forward(&a, q, k, v, query_lengths, key_lengths, o, logsumexp,
-                                                 workspace(h2x_attention_forward_workspace_bytes(&a)), m_stream));
+                                                 m_workspace.get(h2x_attention_forward_workspace_bytes(&a)), m_stream));
         return 0;
     }
 
@@ -154,22 +176,13 @@ public:
                  const int32_t* key_lengths = nullptr)
     {
         DISTCONV_CHECK_H2X(h2x_attention_backward(&a, q, k, v, o, d_o, logsumexp, query_lengths, key_lengths, dq, dk, dv,
-                                                  workspace(h2x_attention_backward_workspace_bytes(&a)), m_stream));
+                                                  m_workspace.get(h2x_attention_backward_workspace_bytes(&a)), m_stream));
         return 0;
     }
 
 private:
-    void* workspace(size_t bytes)
-    {
-        if (bytes == 0)
-            return nullptr;
-        if (m_workspace.is_null() || m_workspace.get_size() < bytes)
-            m_workspace.allocate(bytes);
-        return m_workspace.get();
-    }
-
     hipStream_t m_stream;
-    tensor::Memory<tensor::CUDAAllocator> m_workspace;
+    TokenWorkspace m_workspace;
 };
 
 } // namespace distconv

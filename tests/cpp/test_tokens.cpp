@@ -2,6 +2,8 @@
 // in double.  Errors are compared with 1e-5 of the results' root mean square: sums of at most a hundred terms in 32 bits, 100 * 2^-24 = 6e-6.
 #include "test_common.hpp"
 
+#include <algorithm>
+
 static std::vector<float> randn(size_t n, unsigned seed)
 {
     std::mt19937 gen(seed);
@@ -202,9 +204,63 @@ static int test_attention()
     return errors;
 }
 
+// A captured backward pass replays with the workspace that it was captured with, though larger calls of the layer followed.
+static int test_graph()
+{
+    const int most = 160, heads = 2, dim = 8;
+    const size_t size = most * heads * dim;
+    const auto hq = randn(size, 10), hk = randn(size, 11), hv = randn(size, 12), hd = randn(size, 13);
+    Buffer<float> q(hq), k(hk), v(hv), d_o(hd), o(size), dq(size), dk(size), dv(size), lse(heads * most);
+    h2x_attention a = {};
+    a.dtype = H2X_F32;
+    a.head_dim = dim;
+    a.samples = 1;
+    a.query_heads = a.key_heads = heads;
+    a.window_left = -1;
+    a.scale = 0.3;
+    a.q = a.o = a.d_o = a.dq = a.k = a.v = a.dk = a.dv = {0, heads * dim, dim};
+    hipStream_t stream;
+    DISTCONV_CHECK_HIP(hipStreamCreateWithFlags(&stream, hipStreamNonBlocking));
+    DISTCONV_CHECK_HIP(hipDeviceSynchronize());
+    int errors = 0;
+    {
+        BackendMI355X backend(stream);
+        Attention<BackendMI355X> layer(backend);
+        const auto run = [&](int tokens) {
+            a.queries = a.keys = tokens;
+            layer.forward(a, q.p, k.p, v.p, o.p, lse.p);
+            layer.backward(a, q.p, k.p, v.p, o.p, d_o.p, lse.p, dq.p, dk.p, dv.p);
+        };
+        run(40);
+        const auto want_q = dq.host(), want_k = dk.host(), want_v = dv.host();
+        hipGraph_t graph;
+        hipGraphExec_t replay;
+        DISTCONV_CHECK_HIP(hipStreamBeginCapture(stream, hipStreamCaptureModeThreadLocal));
+        run(40);
+        DISTCONV_CHECK_HIP(hipStreamEndCapture(stream, &graph));
+        DISTCONV_CHECK_HIP(hipGraphInstantiate(&replay, graph, nullptr, nullptr, 0));
+        for (int i = 0; i < 3; ++i)
+        {
+            run(most); // (the first one needs a larger workspace)
+            DISTCONV_CHECK_HIP(hipGraphLaunch(replay, stream));
+            DISTCONV_CHECK_HIP(hipStreamSynchronize(stream));
+            const auto same = [&](const Buffer<float>& b, const std::vector<float>& want) {
+                const auto got = b.host();
+                return std::equal(got.begin(), got.begin() + 40 * heads * dim, want.begin());
+            };
+            errors += !(same(dq, want_q) && same(dk, want_k) && same(dv, want_v));
+        }
+        DISTCONV_CHECK_HIP(hipGraphExecDestroy(replay));
+        DISTCONV_CHECK_HIP(hipGraphDestroy(graph));
+    }
+    DISTCONV_CHECK_HIP(hipStreamDestroy(stream));
+    std::printf("captured attention %s\n", errors ? "FAILED" : "ok");
+    return errors;
+}
+
 int main()
 {
-    const int errors = test_norm() + test_rotary() + test_attention();
+    const int errors = test_norm() + test_rotary() + test_attention() + test_graph();
     std::printf(errors ? "test_tokens: %d FAILED\n" : "test_tokens: ok\n", errors);
     return finish(errors);
 }
