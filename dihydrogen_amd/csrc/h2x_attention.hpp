@@ -77,11 +77,6 @@ enum Order
     kFirstFirst, // the first blocks of all heads, which have the most to do, then the second ones ...
     kLastFirst   // the same from the last ones on
 };
-struct Schedule
-{
-    Order order;
-    int fold; // blocks from this one on come the other way round
-};
 
 #ifdef __HIPCC__
 
@@ -90,23 +85,21 @@ struct Place
     int head, block; // the head counted through all samples
 };
 // Of workgroup `id` of a grid of `grid`; heads from `heads` on have nothing to do.
-__device__ __forceinline__ Place place_of(const Schedule& s, uint32_t id, uint32_t grid, uint32_t heads, uint32_t blocks)
+__device__ __forceinline__ Place place_of(Order order, uint32_t id, uint32_t grid, uint32_t heads, uint32_t blocks)
 {
-    if (s.order == kByHead)
+    if (order == kByHead)
     {
         id = xcd_contiguous(id, grid);
         const uint32_t head = id / blocks;
         return {static_cast<int>(head), static_cast<int>(id - head * blocks)};
     }
-    uint32_t block = id / heads;
+    const uint32_t block = id / heads;
     const uint32_t at = id - block * heads;
     if (block >= blocks)
         return {static_cast<int>(heads), 0};
-    if (block >= static_cast<uint32_t>(s.fold))
-        block = s.fold + blocks - 1 - block;
     // workgroups of heads next to each other on one XCD, where the number of heads allows it
     const uint32_t head = heads % kNumXcd == 0 ? at % kNumXcd * (heads / kNumXcd) + at / kNumXcd : at;
-    return {static_cast<int>(head), static_cast<int>(s.order == kFirstFirst ? block : blocks - 1 - block)};
+    return {static_cast<int>(head), static_cast<int>(order == kFirstFirst ? block : blocks - 1 - block)};
 }
 
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -641,14 +634,11 @@ inline Masks masks_of(const h2x_attention& a, const int32_t* query_lengths, cons
 }
 
 // The order for blocks of queries, or of keys, which are the other way round.  Under a mask that bounds one side blocks have unlike numbers of
-// tiles: the longest first, so that the short ones fill up the end.  Where all workgroups run at once, two a CU, the second one of a CU is the
-// shorter the longer its first.
-inline Schedule schedule_of(const h2x_attention& a, bool keys, uint64_t heads, uint64_t blocks)
+// tiles: the longest first, so that the short ones fill up the end.
+inline Order order_of(const h2x_attention& a, bool keys)
 {
     const bool left = a.window_left >= 0, right = a.window_right >= 0;
-    if (left == right)
-        return {kByHead, 0};
-    return {right != keys ? kLastFirst : kFirstFirst, static_cast<int>(blocks)};
+    return left == right ? kByHead : right != keys ? kLastFirst : kFirstFirst;
 }
 
 // Elements of a head in LDS, a multiple of 32, and in a contraction, of 16.

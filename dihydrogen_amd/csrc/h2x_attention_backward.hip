@@ -51,7 +51,7 @@ struct Args
     float scale, scale_log2;
     int dim, query_heads, group;
     int blocks, heads; // of rows in a head, and heads in all samples
-    Schedule schedule;
+    Order order;
     // The other side's tiles of a block of rows are shared by `parts` workgroups (1: one writes the gradients).  Part p's sums for row r, of `rows`, lie
     // at (p * rows + r) * padded_dim, those for the values behind those for the keys.
     int parts;
@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr int KT = kTileRows<T>, B = KT / 32;
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, KT>];
-    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks * a.parts);
+    const Place place = place_of(a.order, blockIdx.x, gridDim.x, a.heads, a.blocks * a.parts);
     if (place.head >= a.heads)
         return;
     const int block = place.block / a.parts, part = place.block - block * a.parts;
@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, QT>];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kWaveSize];
     const int key_heads = a.query_heads / a.group;
-    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.blocks * a.parts);
+    const Place place = place_of(a.order, blockIdx.x, gridDim.x, a.heads, a.blocks * a.parts);
     if (place.head >= a.heads)
         return;
     const int block = place.block / a.parts, part = place.block - block * a.parts;
@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kThreads, (DP == 128 ? 1 : kWavesOf<T, DP, Who
             const int at = here + 32 * b0;
             if (first > last || at >= some_end || at + 32 * N <= some_from)
                 continue;
-            // All blocks of the tile in one go: the products of one run beside the exponentials of another.
+            // (Where two blocks are taken in one go, the products of one run beside the exponentials of the other.)
             f32x16 s[N], dp[N];
             products<T, DP, DQ, QT>(q_tile, 32 * b0, k, s);
             products<T, DP, DQ, QT>(d_o_tile, 32 * b0, v, dp);
@@ -442,7 +442,7 @@ int issue(const h2x_attention& c, const Plan& p, Args<T> a, hipStream_t stream)
             a.blocks = static_cast<int>(p.query_blocks);
             a.heads = static_cast<int>(query_heads);
             a.parts = p.query_parts;
-            a.schedule = schedule_of(c, false, a.heads, p.query_blocks * p.query_parts);
+            a.order = order_of(c, false);
             launch(attention_dq_kernel<T, DP, DQ, Whole>, grid(query_groups), dim3(kThreads), stream, a);
             if (a.parts > 1)
             {
@@ -460,7 +460,7 @@ int issue(const h2x_attention& c, const Plan& p, Args<T> a, hipStream_t stream)
             a.blocks = static_cast<int>(p.key_blocks);
             a.heads = static_cast<int>(key_heads);
             a.parts = p.key_parts;
-            a.schedule = schedule_of(c, true, a.heads, p.key_blocks * p.key_parts);
+            a.order = order_of(c, true);
             launch(attention_dkv_kernel<T, DP, DQ, Whole>, grid(key_groups), dim3(kThreads), stream, a);
             if (a.parts > 1)
             {

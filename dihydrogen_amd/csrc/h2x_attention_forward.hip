@@ -35,7 +35,7 @@ struct Args
     float scale_log2;
     int dim, samples, query_heads, group, query_blocks;
     int heads; // of all samples; with split keys key heads
-    Schedule schedule;
+    Order order;
 };
 
 // A wave's 32 rows.
@@ -124,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 2 || DP <= 96 ? 2 : 1)
 #ifdef __HIP_DEVICE_COMPILE__
     constexpr int KT = kTileKeys<T>;
     __shared__ __attribute__((aligned(16))) char lds[2][2][kTileBytes<T, DP, KT>];
-    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.query_blocks);
+    const Place place = place_of(a.order, blockIdx.x, gridDim.x, a.heads, a.query_blocks);
     if (place.head >= a.heads)
         return;
     const int block = place.block, n = place.head / a.query_heads, head = place.head - n * a.query_heads;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kThreads) attention_split_kernel(const Args<T>
     constexpr int kJoinStride = DP + 4, kJoinBytes = kWaves * kRows * kJoinStride * 4;
     __shared__ __attribute__((aligned(16))) char lds[kTilesBytes > kJoinBytes ? kTilesBytes : kJoinBytes];
     __shared__ float max_sum[kWaves][kRows][2];
-    const Place place = place_of(a.schedule, blockIdx.x, gridDim.x, a.heads, a.query_blocks * a.parts.num);
+    const Place place = place_of(a.order, blockIdx.x, gridDim.x, a.heads, a.query_blocks * a.parts.num);
     if (place.head >= a.heads)
         return;
     const int key_heads = a.query_heads / a.group;
@@ -555,7 +555,7 @@ extern "C" int h2x_attention_forward(const h2x_attention* attention, const void*
         a.group = c.query_heads / c.key_heads;
         a.query_blocks = p.query_blocks;
         a.heads = c.samples * (p.split ? c.key_heads : c.query_heads);
-        a.schedule = schedule_of(c, false, a.heads, static_cast<uint64_t>(p.query_blocks) * p.parts);
+        a.order = order_of(c, false);
         return issue<T, decltype(is_whole)::value>(c, p, a, as_stream(stream));
     });
 }

@@ -1,6 +1,6 @@
 """Calls of the token operators that have to be refused, by the C ABI before any launch and by the Python
 layers with an error that says why.  (No kernel runs: pointers are imaginary, and the file is skipped where a GPU is
-visible; tests/test_gpu_token_refusals.py has the twin with real buffers.)"""
+visible.)"""
 import ctypes
 
 import pytest
