@@ -244,3 +244,15 @@ def test_most_channels():
     bwd = lambda c: lib.h2x_layer_norm_backward(capi.F32, capi.F32, 1, c, None, None, None, P, P, P, P, P, O, P, P, P, None)
     for call in (fwd, bwd):
         assert call(most) > 0 and call(most + 1) == TOO_LARGE and call(1 << 26) == TOO_LARGE
+
+
+def test_more_heads_than_any_grid_has():
+    """Products of the sizes that pass 64 bits are refused, not wrapped."""
+    lib, most = capi.load(), 2 ** 31 - 1
+    for samples, heads, queries in ((1 << 30, 1 << 30, 1 << 4), (most, most, most - 256), (1 << 16, 1 << 16, 1 << 30), (1, most, most - 256)):
+        a = _attention(samples=samples, query_heads=heads, key_heads=heads, queries=queries)
+        for name in ("q", "k", "v", "o", "d_o", "dq", "dk", "dv"):
+            setattr(a, name, capi.TokenStrides(64, 64, 64))
+        p = [ctypes.c_void_p((i + 1) << 20) for i in range(9)]
+        assert lib.h2x_attention_forward(ctypes.byref(a), *p[:3], None, None, p[3], P, P, None) == TOO_LARGE
+        assert lib.h2x_attention_backward(ctypes.byref(a), *p[:5], P, None, None, *p[5:8], P, None) == TOO_LARGE
