@@ -131,7 +131,7 @@ __global__ void __launch_bounds__(kThreads, (kWavesOf<T, DP, Whole>)) attention_
     if (there)
     {
         const float l = a.logsumexp[row];
-        if (l > -INFINITY)
+        if (l != -INFINITY) // (one that is NaN is no empty row's)
             log2_sum = l * kLog2e;
         if (lane < 32 && part == 0)
         {

@@ -16,7 +16,8 @@ template <typename T>
 constexpr int kTileKeys = sizeof(T) == 2 ? 64 : 32;
 
 // What parts of the keys give, to be joined: for part p and row r (of samples * query_heads * queries), the unnormalised output at
-// (p * rows + r) * padded_dim, and the row's maximum and sum at 2 (p * rows + r).
+// (p * rows + r) * padded_dim, and the row's maximum and sum at 2 (p * rows + r).  The maximum of a row that sees no key of any part is minus
+// infinity; of one that sees some it is finite in parts where it sees none.
 struct Parts
 {
     float *out, *max_sum;
@@ -193,13 +194,12 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 2 || DP <= 96 ? 2 : 1)
     }
     if (i < a.masks.queries)
     {
-        const bool there = i < sample.queries;
+        const bool sees = i < sample.queries && rows.from < rows.end; // (its sum may still be anything, NaN among them)
         const float sum = halves_sum(rows.sum);
-        store_row<T, DP, Whole>(a.o + n * a.os.sample + head * a.os.head + i * a.os.token, a.dim, rows.out,
-                                there && sum > 0.0f ? 1.0f / sum : 0.0f);
+        store_row<T, DP, Whole>(a.o + n * a.os.sample + head * a.os.head + i * a.os.token, a.dim, rows.out, sees ? 1.0f / sum : 0.0f);
         if (a.logsumexp && lane < 32)
             a.logsumexp[(static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + i] =
-                there && sum > 0.0f ? (rows.max + log2f(sum)) * kLn2 : -INFINITY;
+                sees ? (rows.max + log2f(sum)) * kLn2 : -INFINITY;
     }
 #endif
 }
@@ -322,24 +322,24 @@ __global__ void __launch_bounds__(kThreads) attention_split_kernel(const Args<T>
     if (first + row > last)
         return;
     const int my_head = (first + row) / queries, my_query = first + row - my_head * queries;
-    const bool mine = my_query < sample.queries;
-    if (!mine)
+    const bool sees = my_query < sample.queries && sample.first_key(my_query) < sample.end_key(my_query);
+    if (!sees)
         total = 0.0f;
     const int64_t at = (static_cast<int64_t>(n) * a.query_heads + key_head * a.group + my_head) * queries + my_query;
     const int64_t all = static_cast<int64_t>(a.samples) * a.query_heads * queries;
     const bool whole = a.parts.num == 1;
     T* const o = a.o + n * a.os.sample + (key_head * a.group + my_head) * a.os.head + my_query * a.os.token;
     float* const share = a.parts.out + (part * all + at) * DP;
-    const float scale = total > 0.0f ? 1.0f / total : 0.0f;
+    const float scale = sees ? 1.0f / total : 0.0f;
     if (column == 0)
     {
         if (!whole)
         {
-            a.parts.max_sum[2 * (part * all + at)] = max;
+            a.parts.max_sum[2 * (part * all + at)] = sees ? max : -INFINITY;
             a.parts.max_sum[2 * (part * all + at) + 1] = total;
         }
         else if (a.logsumexp)
-            a.logsumexp[at] = total > 0.0f ? (max + log2f(total)) * kLn2 : -INFINITY;
+            a.logsumexp[at] = sees ? (max + log2f(total)) * kLn2 : -INFINITY;
     }
 #pragma unroll
     for (int d = 4 * column; d < DP; d += 32)
@@ -383,7 +383,8 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const Args<T> 
         max = a.parts.max_sum[2 * (lane * rows + row)];
         sum = a.parts.max_sum[2 * (lane * rows + row) + 1];
     }
-    const bool any = sum > 0.0f; // (where no key was seen the output was not written)
+    const bool sees = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(max))) > -INFINITY; // (lane 0 has the first part)
+    const bool any = !(sum == 0.0f); // (a part without keys counts nothing; one whose sum is NaN makes all NaN)
     const float most = wave_combine(any ? max : kLowest, [](float x, float y) { return fmaxf(x, y); });
     const float factor = any ? __builtin_amdgcn_exp2f(max - most) : 0.0f;
     factors[wave][lane] = factor;
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const Args<T> 
         for (int n = 0; n < N; ++n)
         {
             const float x = n * kWaveSize + lane < DP ? a.parts.out[(p * rows + row) * DP + n * kWaveSize + lane] : 0.0f;
-            out[n] = f > 0.0f ? __builtin_fmaf(x, f, out[n]) : out[n];
+            out[n] = f != 0.0f ? __builtin_fmaf(x, f, out[n]) : out[n];
         }
     }
     if constexpr (S > 1)
@@ -421,9 +422,9 @@ __global__ void __launch_bounds__(kThreads) attention_join_kernel(const Args<T> 
 #pragma unroll
     for (int e = 0; e < N; ++e)
         if (e * kWaveSize + lane < a.dim)
-            o[e * kWaveSize + lane] = static_cast<T>(sum > 0.0f ? out[e] / sum : 0.0f);
+            o[e * kWaveSize + lane] = static_cast<T>(sees ? out[e] / sum : 0.0f);
     if (a.logsumexp && lane == 0)
-        a.logsumexp[row] = sum > 0.0f ? (most + log2f(sum)) * kLn2 : -INFINITY;
+        a.logsumexp[row] = sees ? (most + log2f(sum)) * kLn2 : -INFINITY;
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------

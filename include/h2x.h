@@ -1435,7 +1435,9 @@ int h2x_rotary_apply(const h2x_rotary* rotary,
  * (window_right = 0: a query sees no key behind its own place).  Keys and values that any query sees have to be finite (floats: below 3e38);
  * what no query sees may hold anything.
  * Empty rows (a query that sees no key, or lies behind its sample's queries) have output zero and a logarithm of minus infinity, and give
- * no gradients; rows of the gradients behind the lengths are zero.
+ * no gradients; rows of the gradients behind the lengths are zero.  A query with a score that is NaN or plus infinity (it holds such numbers, or its
+ * products overflow) has an output and a logarithm of NaN, and its gradients and those of the keys it sees are NaN (those of
+ * other keys may be).
  */
 typedef struct h2x_attention
 {
