@@ -529,6 +529,8 @@ extern "C" int h2x_attention_forward(const h2x_attention* attention, const void*
     const Plan p = plan_of(c);
     if (!q || !o || (c.keys > 0 && (!k || !v || o == k || o == v)) || (p.parts > 1 && !workspace))
         return H2X_ERR_INVALID_ARGUMENT;
+    if (o == q && (os.sample != qs.sample || os.token != qs.token || os.head != qs.head)) // (a workgroup overwrites the rows that it has read, and no others)
+        return H2X_ERR_INVALID_ARGUMENT;
     if (p.groups > 0x800000u || (p.parts > 1 && rows_of(c) > 0x800000u))
         return H2X_ERR_TOO_LARGE; // (a grid of fewer than 2^32 threads)
     const bool whole = whole_rows(c, q, qs) && whole_rows(c, k, ks) && whole_rows(c, v, vs) && whole_rows(c, o, os);

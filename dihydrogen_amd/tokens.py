@@ -335,7 +335,8 @@ class Attention:
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, output: torch.Tensor,
                 logsumexp: Optional[torch.Tensor] = None, query_lengths: Optional[torch.Tensor] = None,
                 key_lengths: Optional[torch.Tensor] = None) -> int:
-        """logsumexp, (samples, heads, queries), is for the backward pass."""
+        """logsumexp, (samples, heads, queries), is for the backward pass.  output may be query itself (the same strides), and overlap no input
+        otherwise."""
         device = _current_device()
         alike = _key(self._calls, device, query, key, value, output, logsumexp, query_lengths, key_lengths)
         address, nbytes, _ = self._plans.get(alike) or self._plan(alike, device, query, key, value, output, logsumexp,

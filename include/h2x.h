@@ -1458,7 +1458,8 @@ size_t h2x_attention_forward_workspace_bytes(const h2x_attention* attention);
 /**
  * s = scale * q k^T;  p = exp(s - logsumexp) where a query sees a key;  o = p v;  logsumexp = log sum exp s, in 32 bits, at
  * (sample * query_heads + head) * queries + query, or NULL.  Scores, sums and outputs are accumulated in 32 bits; with
- * H2X_BF16 the probabilities are rounded to 16 bits for the product with v.
+ * H2X_BF16 the probabilities are rounded to 16 bits for the product with v.  o may be q itself, with the same strides; it may not overlap inputs
+ * otherwise.
  */
 int h2x_attention_forward(const h2x_attention* attention,
                           const void* q,
