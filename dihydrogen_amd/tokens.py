@@ -197,7 +197,8 @@ def grid_positions(tensor: Tensor, dims: Optional[Sequence[int]] = None) -> torc
 class RotaryPositions:
     """Turns pairs of a head's elements by angles that grow with a token's position: pair i of an axis
     with m pairs by position * base ** (-i / m).  ``axis_pairs``: how many pairs belong to each axis (time or depth, height, width); elements
-    behind the pairs are copied.  ``frequencies``, a float64 tensor of one a pair, may be replaced before the first call.
+    behind the pairs are copied.  ``frequencies``, a float64 tensor of one a pair, may be replaced before the first call, which copies it to the
+    GPU; head_dim, axis_pairs and pairing are the layer's for good.
 
     x: (samples, tokens, heads, head_dim), float32, float64, bfloat16 or float16.  positions: int32, (axes, tokens) for all
     samples or (samples, axes, tokens), tokens contiguous; see grid_positions().
@@ -205,22 +206,52 @@ class RotaryPositions:
 
     def __init__(self, head_dim: int, axis_pairs: Sequence[int], base: float = 10000.0,
                  pairing: RotaryPairing = RotaryPairing.HALVES, stream: Optional[torch.cuda.Stream] = None):
-        self.head_dim, self.axis_pairs, self.pairing, self.stream = int(head_dim), [int(m) for m in axis_pairs], pairing, stream
+        self._head_dim, self._axis_pairs, self._pairing = int(head_dim), tuple(int(m) for m in axis_pairs), RotaryPairing(pairing)
+        self.stream = stream
         _require(1 <= len(self.axis_pairs) <= capi.MAX_AXES and min(self.axis_pairs) >= 0, f"1 to {capi.MAX_AXES} axes")
         _require(1 <= 2 * sum(self.axis_pairs) <= self.head_dim, "the pairs of all axes have to fit a head")
         _require(base > 0, "base has to be positive")
+        self._on_device = {}  # the frequencies, by the index of a GPU
         self.frequencies = torch.tensor([float(base) ** (-i / m) for m in self.axis_pairs for i in range(m)],
                                         dtype=torch.float64)
         self._calls = capi.calls()
         self._plans = _Plans()
-        self._on_device = {}  # the frequencies, by the index of a GPU
+
+    # (fixed: plans are made with them, and kernels read a frequency for each pair)
+    @property
+    def head_dim(self) -> int:
+        return self._head_dim
+
+    @property
+    def axis_pairs(self) -> Tuple[int, ...]:
+        return self._axis_pairs
+
+    @property
+    def pairing(self) -> RotaryPairing:
+        return self._pairing
+
+    @property
+    def frequencies(self) -> torch.Tensor:
+        return self._given_frequencies
+
+    @frequencies.setter
+    def frequencies(self, given: torch.Tensor) -> None:
+        _require(not self._on_device, "the frequencies have been copied to a GPU by the first call there")
+        self._check_frequencies(given)
+        self._given_frequencies = given
+
+    def _check_frequencies(self, given: torch.Tensor) -> None:
+        _require(isinstance(given, torch.Tensor) and given.dtype == torch.float64 and tuple(given.shape) == (sum(self.axis_pairs),),
+                 f"frequencies: float64, one for each of the {sum(self.axis_pairs)} pairs")
 
     def _frequencies(self, device: torch.device) -> torch.Tensor:
         kept = self._on_device.get(device.index)
         if kept is None:
+            self._check_frequencies(self.frequencies)  # (a tensor can be resized where it is)
             _require(not torch.cuda.is_current_stream_capturing(),
                      "the first call on a GPU copies the frequencies there: make one before a graph is captured")
-            kept = self._on_device[device.index] = self.frequencies.to(device)
+            own = torch.empty(len(self.frequencies), dtype=torch.float64, device=device)
+            kept = self._on_device[device.index] = own.copy_(self.frequencies.detach())  # (whatever its strides were)
             torch.cuda.current_stream(device).synchronize()  # whatever stream comes next finds them
         return kept
 
