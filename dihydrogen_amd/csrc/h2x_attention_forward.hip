@@ -196,7 +196,13 @@ __global__ void __launch_bounds__(kThreads, (sizeof(T) == 2 || DP <= 96 ? 2 : 1)
     {
         const bool sees = i < sample.queries && rows.from < rows.end; // (its sum may still be anything, NaN among them)
         const float sum = halves_sum(rows.sum);
-        store_row<T, DP, Whole>(a.o + n * a.os.sample + head * a.os.head + i * a.os.token, a.dim, rows.out, sees ? 1.0f / sum : 0.0f);
+        if (!sees) // (a query of zeros, whose sums may have overflowed)
+        {
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+                rows.out[d] = zero16();
+        }
+        store_row<T, DP, Whole>(a.o + n * a.os.sample + head * a.os.head + i * a.os.token, a.dim, rows.out, 1.0f / (sees ? sum : 1.0f));
         if (a.logsumexp && lane < 32)
             a.logsumexp[(static_cast<int64_t>(n) * a.query_heads + head) * a.masks.queries + i] =
                 sees ? (rows.max + log2f(sum)) * kLn2 : -INFINITY;
@@ -330,7 +336,7 @@ __global__ void __launch_bounds__(kThreads) attention_split_kernel(const Args<T>
     const bool whole = a.parts.num == 1;
     T* const o = a.o + n * a.os.sample + (key_head * a.group + my_head) * a.os.head + my_query * a.os.token;
     float* const share = a.parts.out + (part * all + at) * DP;
-    const float scale = sees ? 1.0f / total : 0.0f;
+    const float scale = 1.0f / total;
     if (column == 0)
     {
         if (!whole)
@@ -361,7 +367,7 @@ __global__ void __launch_bounds__(kThreads) attention_split_kernel(const Args<T>
 #pragma unroll
         for (int j = 0; j < 4; ++j)
             if (d + j < a.dim)
-                o[d + j] = static_cast<T>(x[j] * scale);
+                o[d + j] = static_cast<T>(sees ? x[j] * scale : 0.0f); // (a query of zeros may have sums that overflowed)
     }
 #endif
 }

@@ -307,7 +307,8 @@ class Attention:
     own place to `right` behind it; None: no bound.  ``causal``: no key behind its own place.
     ``query_lengths``, ``key_lengths``: int32 on the GPU, one a sample, for padded batches and caches; None: samples are whole.  Rows behind a
     sample's lengths are not read; their outputs and gradients are zero, as are those of queries that see no key, whose logsumexp is minus infinity.
-    Keys and values that any query sees have to be finite (float32: below 3e38).  A query with a score that is NaN or plus infinity has an
+    Keys and values that any query sees have to be finite (float32: below 3e38), and values times 2^8 times the number of keys below 2^128 (sums are
+    in 32 bits, and divided at the end).  A query with a score that is NaN or plus infinity has an
     output and a logsumexp of NaN.
     """
 

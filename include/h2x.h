@@ -1433,7 +1433,9 @@ int h2x_rotary_apply(const h2x_rotary* rotary,
  * Mask: the last query of a sample stands at its last key, so query i stands at place(i) = i + its keys - its queries, and sees the keys
  * j with place(i) - window_left <= j <= place(i) + window_right; a negative window_left or window_right has no bound
  * (window_right = 0: a query sees no key behind its own place).  Keys and values that any query sees have to be finite (floats: below 3e38);
- * what no query sees may hold anything.
+ * what no query sees may hold anything.  Sums are in 32 bits, of products of probabilities that are divided by their sum at the end, and that may
+ * be up to 2^8 until then: the number of keys that a query sees times the largest value times 2^8 has to stay below 2^128 (1000 keys: values up to 1e33),
+ * in the backward pass sums of the products that its formulas name.
  * Empty rows (a query that sees no key, or lies behind its sample's queries) have output zero and a logarithm of minus infinity, and give
  * no gradients; rows of the gradients behind the lengths are zero.  A query with a score that is NaN or plus infinity (it holds such numbers, or its
  * products overflow) has an output and a logarithm of NaN, and its gradients and those of the keys it sees are NaN (those of
