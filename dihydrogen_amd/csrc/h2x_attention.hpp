@@ -594,7 +594,8 @@ inline int check(const h2x_attention* a)
         return H2X_ERR_INVALID_ARGUMENT;
     if (a->head_dim > 128)
         return H2X_ERR_UNSUPPORTED;
-    if (a->queries > 0x7fffffff - 256 || a->keys > 0x7fffffff - 256 || static_cast<int64_t>(a->samples) * a->query_heads > 0x7fffffff)
+    const int64_t heads = a->query_heads > 0 ? a->query_heads : a->key_heads; // (query heads are no fewer where there are any)
+    if (a->queries > 0x7fffffff - 256 || a->keys > 0x7fffffff - 256 || a->samples * heads > 0x7fffffff)
         return H2X_ERR_TOO_LARGE;
     return H2X_SUCCESS;
 }

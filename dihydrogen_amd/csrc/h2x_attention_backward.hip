@@ -489,7 +489,7 @@ using namespace h2x::attention;
 extern "C" size_t h2x_attention_backward_workspace_bytes(const h2x_attention* attention)
 {
     if (check(attention) != H2X_SUCCESS || attention->samples == 0 || attention->query_heads == 0)
-        return 0;
+        return 0; // (without query heads: zeros alone are written)
     return plan_of(*attention).bytes;
 }
 
@@ -500,7 +500,7 @@ extern "C" int h2x_attention_backward(const h2x_attention* attention, const void
 {
     if (const int bad = check(attention))
         return bad;
-    const h2x_attention& c = *attention;
+    h2x_attention c = *attention;
     struct Operand
     {
         const void* p;
@@ -520,9 +520,14 @@ extern "C" int h2x_attention_backward(const h2x_attention* attention, const void
         if (const int bad = check_strides(c, x.s, x.tokens, x.heads, x.output))
             return bad;
         whole = whole && whole_rows(c, x.p, x.s);
-        missing = missing || (!x.p && x.tokens > 0);
+        missing = missing || (!x.p && x.tokens > 0 && x.heads > 0);
     }
-    if (c.samples == 0 || c.query_heads == 0 || (c.queries == 0 && c.keys == 0))
+    if (c.query_heads == 0) // keys have the gradients that they have from no queries
+    {
+        c.query_heads = c.key_heads;
+        c.queries = 0;
+    }
+    if (c.samples == 0 || c.key_heads == 0 || (c.queries == 0 && c.keys == 0))
         return H2X_SUCCESS;
     for (int out = 5; out < 8; ++out) // the second kernel reads what the first would have overwritten
         for (int x = 0; x < out; ++x)

@@ -1480,7 +1480,7 @@ size_t h2x_attention_backward_workspace_bytes(const h2x_attention* attention);
 /**
  * Gradients, recomputing p from logsumexp; with delta = sum over a head's elements of d_o * o:
  *   dv = p^T d_o;  ds = p (d_o v^T - delta);  dq = scale * ds k;  dk = scale * ds^T q;
- * dk and dv of a key head are sums over the query heads that share it.  o, logsumexp: of the forward pass.  Every sum is
+ * dk and dv of a key head are sums over the query heads that share it (zero without query heads).  o, logsumexp: of the forward pass.  Every sum is
  * made in a fixed order.  Outputs may not overlap inputs.
  */
 int h2x_attention_backward(const h2x_attention* attention,
