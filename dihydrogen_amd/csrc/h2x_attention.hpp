@@ -286,15 +286,20 @@ constexpr unsigned int kOutside = 0x80000000u; // behind every buffer
 // all loads that its own form of these has issued before it reads any LDS across, those for the next tile among them (gradients of keys,
 // heads of 128: 674 us, 550 without loads).  Nothing is returned to registers; who reads the LDS waits with wait_for_loads().  (Five wait states
 // between a lane's number put into a scalar register and a load that uses it, one after m0: the compiler does not see to that in assembly.)
+// m0 is named as written, so that the compiler keeps no number of its own there from before to behind; it warns that it saves none either.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 template <int Bytes>
 __device__ __forceinline__ void load_to_lds(const u32x4& b, unsigned int at, LdsBytes to)
 {
     const int place = __builtin_amdgcn_readfirstlane(static_cast<int>(reinterpret_cast<uintptr_t>(to)));
     if constexpr (Bytes == 16)
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(place), "v"(at), "s"(b) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(place), "v"(at), "s"(b) : "memory", "m0");
     else
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(place), "v"(at), "s"(b) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dword %1, %2, 0 offen lds" ::"s"(place), "v"(at), "s"(b) : "memory", "m0");
 }
+
+#pragma clang diagnostic pop
 
 // Until no more than N of this wave's loads are under way (they arrive in order).
 template <int N = 0>
