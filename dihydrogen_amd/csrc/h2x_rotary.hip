@@ -2,7 +2,8 @@
 //
 // Bound by memory: every element is read and written once.  An angle belongs to a token and a pair, not to a head, so a
 // thread makes the sine and cosine of its pairs once and turns the same pairs of many heads with them.  Angles are made in 64
-// bits and brought to a fraction of a turn there: at position 2^20 an angle in 32 bits is off by 0.06.
+// bits and brought to a fraction of a turn there: at position 2^20 an angle in 32 bits is off by 0.06.  Sine and cosine of that
+// are taken in 32 bits (64 for doubles).
 #include "h2x_token.hpp"
 
 namespace h2x
@@ -32,13 +33,21 @@ struct Turn
     uint64_t first; // workgroups before the launch
 };
 
-// Sine and cosine of position * frequency.
+// Sine and cosine of position * frequency.  At positions of 31 bits a rounding of the angle, or of the turns that it makes, is 2^-25 of a turn and
+// more, three steps of a sine: the product and 1 / (2 pi) are taken in two numbers each.  What is left, within half a turn, fits 32 bits to
+// 2^-26 of a turn (a sine of 1.6 * 2^-24); the part that does not, x, is turned by after sine and cosine: s + x c and c - x s, whose next terms are x^2 /
+// 2 = 2^-48.
 __device__ __forceinline__ void sine_cosine(double position, double frequency, float* s, float* c)
 {
-    const double turns = position * frequency * 0.15915494309189533577;
-    // what is left of the angle, within half a turn, fits 32 bits to 2^-26 of a turn
-    const float rest = static_cast<float>(turns - rint(turns));
-    sincospif(2.0f * rest, s, c);
+    constexpr double kPerTurn = 0.15915494309189535, kPerTurnRest = -9.839338337591243e-18; // 1 / (2 pi)
+    const double angle = position * frequency, angle_rest = __builtin_fma(position, frequency, -angle);
+    const double whole = rint(angle * kPerTurn);
+    const double turns = __builtin_fma(angle, kPerTurn, -whole) + __builtin_fma(angle, kPerTurnRest, angle_rest * kPerTurn);
+    const float rest = static_cast<float>(turns), x = static_cast<float>((turns - rest) * 6.283185307179586);
+    float sine, cosine;
+    sincospif(2.0f * rest, &sine, &cosine);
+    *s = __builtin_fmaf(x, cosine, sine);
+    *c = __builtin_fmaf(-x, sine, cosine);
 }
 __device__ __forceinline__ void sine_cosine(double position, double frequency, double* s, double* c)
 {

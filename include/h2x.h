@@ -1414,7 +1414,8 @@ typedef struct h2x_rotary
 /**
  * Turns the heads of x by their positions into y; inverse != 0: by minus the angles, which is the gradient of the turn.
  * positions: int32 on the device.  frequencies: doubles on the device, one for each pair, radians a step.  Angles are made
- * in 64 bits, at positions of 31 bits too.  y may be x itself, with the same strides.
+ * in 64 bits and brought to a fraction of a turn there, at positions of 31 bits too; their sines and cosines are in 32 bits, right to three
+ * steps of 2^-24 (in 64 with H2X_F64, whose angles carry half a step of their own magnitude).  y may be x itself, with the same strides.
  */
 int h2x_rotary_apply(const h2x_rotary* rotary,
                      const void* x,
