@@ -29,6 +29,12 @@ def _require(condition: bool, what: str) -> None:
         raise ValueError(what)
 
 
+def _require_int32(**counts: int) -> None:
+    """Counts that the C ABI takes in 32 bits, where larger ones would wrap."""
+    for what, n in counts.items():
+        _require(n < 1 << 31, f"{what.replace('_', ' ')}: fewer than 2^31")
+
+
 def _current_device() -> int:
     return torch._C._cuda_getDevice() if _initialized() else _first_device()
 
@@ -117,6 +123,7 @@ class LayerNormalization:
         _require(dtype is not None, f"layer normalisation of {x.dtype} elements is not supported")
         _require(x.dim() >= 1 and x.shape[-1] >= 1, "rows of one element at least")
         channels, rows = x.shape[-1], math.prod(x.shape[:-1])
+        _require_int32(channels=channels)
         for t in others:
             _require(t.shape == x.shape and t.dtype == x.dtype, "tensors of one shape and type")
         given = [w for w in weights if w is not None]
@@ -262,6 +269,7 @@ class RotaryPositions:
         _require_own_memory(y)
         n, tokens, heads, dim = x.shape
         _require(dim == self.head_dim, f"heads of {self.head_dim} elements, not {dim}")
+        _require_int32(samples=n, heads=heads)
         axes = len(self.axis_pairs)
         _require(positions.dtype == torch.int32 and tuple(positions.shape) in ((axes, tokens), (n, axes, tokens)),
                  f"positions: int32, ({axes}, tokens) or (samples, {axes}, tokens)")
@@ -315,7 +323,7 @@ class Attention:
     def __init__(self, scale: Optional[float] = None, causal: bool = False,
                  window: Tuple[Optional[int], Optional[int]] = (None, None), stream: Optional[torch.cuda.Stream] = None):
         left, right = window
-        _require(all(w is None or w >= 0 for w in (left, right)), "a window reaches zero or more keys to either side")
+        _require(all(w is None or 0 <= w < 1 << 63 for w in (left, right)), "a window reaches zero or more keys to either side, below 2^63")
         _require(scale is None or 1e-30 <= scale <= 1e30, "scale has to be positive, from 1e-30 to 1e30")
         if causal:
             _require(right in (None, 0), "a causal window has no keys behind a query's place")
@@ -345,6 +353,7 @@ class Attention:
         _require(k.shape == (n, keys, key_heads, dim) and all(t.shape == k.shape for t in like_k)
                  and all(t.shape == q.shape for t in like_q), "shapes of queries, keys, values and outputs do not fit together")
         _require(1 <= dim <= 128, "heads of 1 to 128 elements")
+        _require_int32(samples=n, heads=heads, key_heads=key_heads)
         _require(heads == 0 or (key_heads > 0 and heads % key_heads == 0), "the number of key heads has to divide that of heads")
         _require(lse is None or (lse.dtype == torch.float32 and lse.shape == (n, heads, queries) and lse.is_contiguous()),
                  "logsumexp: contiguous float32 (samples, heads, queries)")
