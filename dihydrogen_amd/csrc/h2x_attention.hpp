@@ -8,9 +8,11 @@
 // That product contracts over the other side's rows, so its first operand is the same tile in LDS read across, by the
 // transposing LDS loads.
 //
-// Products are of 16-bit numbers, summed in 32 bits.  A float is three of them, each the rounding of what those before it leave: eight bits each,
-// all 24.  Of the nine products of two floats the six that reach 2^-18 of the largest are made; the other three are together below
-// 2^-24, half a step of a float.  Six products of 16-bit numbers take three eighths of the time of one by the matrix units' 32-bit
+// Products are of 16-bit numbers, summed in 32 bits.  Probabilities, and what the backward pass makes of them, are rounded to 16 bits as operands beside
+// elements of 16 bits: half a step of theirs for twice the rate at least; sums of probabilities are of those before the rounding.  A float
+// is three of them, each the rounding of what those before it leave: eight bits each,
+// all 24 (from 2^-109 on, below which the third is no normal number).  Of the nine products of two floats the six that may reach 2^-17 of the
+// largest are made; the other three are together at most 2^-24 of it, half a step of a float, and 2^-34.  Six products of 16-bit numbers take three eighths of the time of one by the matrix units' 32-bit
 // form.
 #pragma once
 

@@ -1438,9 +1438,10 @@ int h2x_rotary_apply(const h2x_rotary* rotary,
  * be up to 2^8 until then: the number of keys that a query sees times the largest value times 2^8 has to stay below 2^128 (1000 keys: values up to 1e33),
  * in the backward pass sums of the products that its formulas name.
  * Empty rows (a query that sees no key, or lies behind its sample's queries) have output zero and a logarithm of minus infinity, and give
- * no gradients; rows of the gradients behind the lengths are zero.  A query with a score that is NaN or plus infinity (it holds such numbers, or its
- * products overflow) has an output and a logarithm of NaN, and its gradients and those of the keys it sees are NaN (those of
- * other keys may be).
+ * no gradients; rows of the gradients behind the lengths are zero.
+ * A query with a score that is NaN or plus infinity (it holds such numbers, or its products overflow) has an output and a logarithm of NaN, one
+ * whose scores all are minus infinity an output of NaN and a logarithm of minus infinity.  The gradients of such a query and of the keys that it sees are
+ * not finite, those of other keys may not be either; and so with a row of d_o that is not finite.
  */
 typedef struct h2x_attention
 {
@@ -1461,7 +1462,8 @@ size_t h2x_attention_forward_workspace_bytes(const h2x_attention* attention);
 /**
  * s = scale * q k^T;  p = exp(s - logsumexp) where a query sees a key;  o = p v;  logsumexp = log sum exp s, in 32 bits, at
  * (sample * query_heads + head) * queries + query, or NULL.  Scores, sums and outputs are accumulated in 32 bits; with
- * H2X_BF16 the probabilities are rounded to 16 bits for the product with v.  o may be q itself, with the same strides; it may not overlap inputs
+ * H2X_BF16 the probabilities are rounded to 16 bits for the product with v; with H2X_F32 numbers are sums of three bfloat16 ones, whose products are
+ * right to 2^-24 for numbers from 2^-109 (1.5e-33) in magnitude on; smaller ones lose bits.  o may be q itself, with the same strides; it may not overlap inputs
  * otherwise.
  */
 int h2x_attention_forward(const h2x_attention* attention,
@@ -1481,6 +1483,8 @@ size_t h2x_attention_backward_workspace_bytes(const h2x_attention* attention);
 /**
  * Gradients, recomputing p from logsumexp; with delta = sum over a head's elements of d_o * o:
  *   dv = p^T d_o;  ds = p (d_o v^T - delta);  dq = scale * ds k;  dk = scale * ds^T q;
+ * with H2X_BF16 p and ds are rounded to 16 bits as factors of p^T d_o, ds k and ds^T q (sums are in 32 bits); with H2X_F32 products are as in the
+ * forward pass.
  * dk and dv of a key head are sums over the query heads that share it (zero without query heads).  o, logsumexp: of the forward pass.  Every sum is
  * made in a fixed order.  Outputs may not overlap inputs.
  */
