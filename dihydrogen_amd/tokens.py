@@ -68,11 +68,12 @@ class _Plans(dict):
         return plan
 
 
-def _key(calls, device: int, *tensors: Optional[torch.Tensor]):
-    """Equal for tensors alike, on the same current device."""
-    key = calls.layout_key(device, *tensors)
+def _key(calls, device: int, stream: Optional[torch.cuda.Stream], *tensors: Optional[torch.Tensor]):
+    """Equal for tensors alike, on the same current device, and streams of the same GPU (a layer's may be replaced)."""
+    where = device if stream is None else device | (stream.device_index + 1) << 16
+    key = calls.layout_key(where, *tensors)
     if key is None:
-        key = (device, *((t.dtype, t.device, t.shape, t.stride()) if t is not None else None for t in tensors))
+        key = (where, *((t.dtype, t.device, t.shape, t.stride()) if t is not None else None for t in tensors))
     return key
 
 
@@ -146,7 +147,7 @@ class LayerNormalization:
     def forward(self, input, scale: Optional[torch.Tensor], bias: Optional[torch.Tensor], output,
                 mean: Optional[torch.Tensor] = None, rstd: Optional[torch.Tensor] = None) -> int:
         x, y, device = _view(input), _view(output), _current_device()
-        key = _key(self._calls, device, x, y, scale, bias, mean, rstd)
+        key = _key(self._calls, device, self.stream, x, y, scale, bias, mean, rstd)
         plan = self._plans.get(key) or self._plan(key, device, (scale, bias), (mean, rstd), x, y)
         dtype, weight_dtype, rows, channels, (xg, yg), _ = plan
         status = self._calls.h2x_layer_norm_forward(dtype, weight_dtype, rows, channels, xg, yg, x, scale, bias, y, mean, rstd,
@@ -159,7 +160,7 @@ class LayerNormalization:
                  scale_gradient: Optional[torch.Tensor] = None, bias_gradient: Optional[torch.Tensor] = None) -> int:
         """Gradients; d_input may be input or d_output itself.  Gradients of scale and bias are overwritten."""
         x, dy, dx, device = _view(input), _view(d_output), _view(d_input), _current_device()
-        key = _key(self._calls, device, x, dy, dx, mean, rstd, scale, scale_gradient, bias_gradient)
+        key = _key(self._calls, device, self.stream, x, dy, dx, mean, rstd, scale, scale_gradient, bias_gradient)
         plan = self._plans.get(key)
         if plan is None:
             _require(mean is not None and rstd is not None, "the backward pass needs mean and rstd")
@@ -286,7 +287,7 @@ class RotaryPositions:
 
     def _apply(self, x: torch.Tensor, positions: torch.Tensor, y: torch.Tensor, inverse: int) -> int:
         device = _current_device()
-        key = _key(self._calls, device, x, positions, y)
+        key = _key(self._calls, device, self.stream, x, positions, y)
         address, alike, _, frequencies = self._plans.get(key) or self._plan(key, device, x, positions, y)
         if not alike:
             _require(x.data_ptr() != y.data_ptr(), "in place: the same strides")
@@ -379,7 +380,7 @@ class Attention:
         """logsumexp, (samples, heads, queries), is for the backward pass.  output may be query itself (the same strides), and overlap no input
         otherwise."""
         device = _current_device()
-        alike = _key(self._calls, device, query, key, value, output, logsumexp, query_lengths, key_lengths)
+        alike = _key(self._calls, device, self.stream, query, key, value, output, logsumexp, query_lengths, key_lengths)
         address, nbytes, _ = self._plans.get(alike) or self._plan(alike, device, query, key, value, output, logsumexp,
                                                                   (query_lengths, key_lengths))
         ws = _buffer_of(self.stream, nbytes, torch.uint8) if nbytes else None
@@ -395,7 +396,8 @@ class Attention:
                  key_lengths: Optional[torch.Tensor] = None) -> int:
         """Gradients, from the forward pass' output and logsumexp; they may not overlap the inputs."""
         device = _current_device()
-        alike = _key(self._calls, device, query, key, value, output, d_output, logsumexp, d_query, d_key, d_value, query_lengths, key_lengths)
+        alike = _key(self._calls, device, self.stream, query, key, value, output, d_output, logsumexp, d_query, d_key, d_value, query_lengths,
+                     key_lengths)
         plan = self._plans.get(alike)
         if plan is None:
             _require(logsumexp is not None, "the backward pass needs logsumexp")
